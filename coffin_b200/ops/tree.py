@@ -58,9 +58,7 @@ def _vec(t: torch.Tensor, n: int, dtype: torch.dtype, name: str) -> None:
 
 
 # ------------------------------------------------------------------ attention
-def tree_splits(nkv: int, rows: int, row_tiles: int, pages: int) -> int:
-    """Splits of the pages so that (kv heads x row tiles x sequences x splits) CTAs cover the SMs."""
-    return max(1, min(pages, 64, 296 // max(1, nkv * rows * row_tiles)))
+CTAS = 148          # pieces that the pages of all sequences are cut into: one CTA an SM
 
 
 def attn_tree(q, proj, kpool, vpool, block_tables, positions, anc, out, *, nh: int, nkv: int, hd: int, kscale=None, vscale=None) -> torch.Tensor:
@@ -89,11 +87,10 @@ def attn_tree(q, proj, kpool, vpool, block_tables, positions, anc, out, *, nh: i
     _place(q, proj=proj, kpool=kpool, vpool=vpool, block_tables=block_tables, positions=positions, anc=anc, out=out, kscale=kscale, vscale=vscale)
     if R == 0:
         return out
-    width = block_tables.shape[1]
-    ns = tree_splits(nkv, R, (C * (nh // nkv) + 63) // 64, width)
-    part = torch.empty(R * C * nh * ns * (hd + 2), dtype=torch.float32, device=q.device)
+    rows = C * (nh // nkv)
+    part = torch.empty((CTAS + R * nkv * -(-rows // 128)) * min(rows, 128) * (hd + 2), dtype=torch.float32, device=q.device)
     call("attn_tree", q, proj, proj.stride(0) if proj is not None else 0, kpool, vpool, slots, kscale, vscale, block_tables, block_tables.stride(0),
-         width, positions, anc, out, out.stride(0), part, R, C, nh, nkv, hd, ns)
+         block_tables.shape[1], positions, anc, out, out.stride(0), part, CTAS, R, C, nh, nkv, hd, K.status_word(q.device))
     K._count(2)
     return out
 
