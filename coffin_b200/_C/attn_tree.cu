@@ -13,10 +13,12 @@
 // slot (CTA + item), which is different for any two segments because one of the two grows from segment to segment.
 //   warp 0       TMA: K and V pages into rings (a page of a kv head is a [64 x hd] box of the pool, hd / 64 swizzled [64 x 128 B] blocks)
 //   warp 1, 10   tcgen05.mma (one thread each): S = Q K^T with Q in tensor memory into one of two accumulators; O += P V
-//   warps 2-9    the segment's Q rows into tensor memory, then the softmax, two threads a row, and the sums out of tensor memory.  The
-//                reference maximum of a row is raised, and O rescaled, only when its maximum has grown by more than 2^8.
-//   warps 11-14  int8 pools, in TMA's place: pages as codes into registers a page ahead, as exact bf16 into the rings.  The keys' scales
-//                multiply the scores, the values' the weights.
+//   warps 2-9    two groups of 128 threads, a thread a row: one takes the even pages, the other the odd ones, so that the exponentials of a
+//                page run under the maxima of the next.  The reference maximum of a row goes from group to group through shared memory
+//                ahead of the exponentials; it is raised, and O rescaled, only when the maximum has grown by more than 2^8.  Between
+//                segments both groups put the next Q rows into tensor memory and take the sums out of it.
+//   warps 11-18  int8 pools, in TMA's place: pages as codes by cp.async, two pages ahead, then as exact bf16 into the rings.  The keys'
+//                scales multiply the scores, the values' the weights.
 // Every wait is bounded by 2 s and reports through the status word; tensor memory is freed on every path.
 #include "sm100.cuh"
 
@@ -24,6 +26,7 @@ namespace {
 using namespace sm100;
 
 constexpr int kPage = 64, kRows = 128, kMaxNodes = 64;
+constexpr int kLoaders = 256;                         // threads that bring int8 pages
 
 struct TreeAttnArgs {
   const bf16* q;                          // [R * C, nh, hd] normed and rotated
@@ -50,13 +53,15 @@ __device__ __forceinline__ int64_t page_slot(const TreeAttnArgs& a, int r, int p
   const int id = a.tables[(int64_t)r * a.ldbt + page];
   return (unsigned)id < (unsigned)a.pages ? (int64_t)id * kPage : -1;
 }
-// The list of all items' pages, cut into even pieces: piece b is [b T / G, (b + 1) T / G).
-__device__ __forceinline__ int64_t piece_start(int64_t b, int64_t T, int G) { return b * T / G; }
-__device__ __forceinline__ int piece_of(int64_t g, int64_t T, int G) { return (int)(((g + 1) * G - 1) / T); }
+// The list of all items' T pages, cut into G even pieces (at most one a page): piece b is [b T / G, (b + 1) T / G).  (64-bit divisions
+// are long: out of line, like everything else here that is not on the path of every page.  See the loaders on the size of the code.)
+__device__ __noinline__ int64_t piece_start(int64_t b, int64_t T, int G) { return b * T / G; }
+__device__ __noinline__ int piece_of(int64_t g, int64_t T, int G) { return (int)(((g + 1) * G - 1) / T); }
 // pages of one item of every sequence before `r`, and of all sequences (a warp)
 __device__ __forceinline__ void page_sums(const TreeAttnArgs& a, int r, int64_t* before, int64_t* all) {
   const int lane = threadIdx.x & 31;
   int64_t b = 0, t = 0;
+#pragma unroll 1
   for (int i = lane; i < a.R; i += 32) {
     const int n = cached_pages(a, i);
     t += n;
@@ -73,76 +78,101 @@ __device__ __forceinline__ void page_sums(const TreeAttnArgs& a, int r, int64_t*
 
 // Segments of a CTA's piece, one after the other.
 struct Segments {
-  int64_t g, end, start;                  // next page of the list, end of the piece, first page of sequence r
-  int r, n;                               // sequence, pages of one of its items
-  int kvh, tile, p0, p1, item;            // the segment: pages [p0, p1) of an item
+  int left;                               // pages of the piece to come
+  int r, n, kvh, tile, item;              // sequence, pages of one of its items, item
+  int p0, p1;                             // the segment: pages [p0, p1) of the item (at first, p1 is where the piece begins)
   __device__ __forceinline__ bool next(const TreeAttnArgs& a) {
-    if (g >= end) return false;
-    const int per = a.nkv * a.tiles;
-    while (g >= start + (int64_t)n * per) {
-      start += (int64_t)n * per;
-      n = cached_pages(a, ++r);
+    if (left <= 0) return false;
+    while (p1 >= n) {
+      p1 = 0;
+      ++item;
+      if (++tile == a.tiles) {
+        tile = 0;
+        if (++kvh == a.nkv) {
+          kvh = 0;
+          n = cached_pages(a, ++r);
+        }
+      }
     }
-    const int64_t at = g - start;
-    const int it = (int)(at / n);
-    p0 = (int)(at - (int64_t)it * n);
-    p1 = (int)min((int64_t)n, p0 + (end - g));
-    kvh = it / a.tiles;
-    tile = it % a.tiles;
-    item = r * per + it;
-    g += p1 - p0;
+    p0 = p1;
+    p1 = min(n, p0 + left);
+    left -= p1 - p0;
     return true;
   }
 };
 
-__device__ __forceinline__ uint64_t tree_now() {
-  uint64_t t;
-  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-  return t;
-}
-__device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
-  if (mbar_try(bar, parity)) return true;
-  const uint64_t t0 = tree_now();
+// Bounded by the SM's own clock, 2 s at its highest rate (the global timer is read over the chip: dozens of warps that wait slow each other).
+__device__ __noinline__ bool tree_wait_long(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  long long t0 = 0;
   for (;;) {
-    for (int i = 0; i < 128; ++i)
+#pragma unroll 1
+    for (int i = 0; i < 64; ++i)
       if (mbar_try(bar, parity)) return true;
     if (*abort_flag) return false;
-    if (tree_now() - t0 > 2000000000ull) return false;
+    const long long now = clock64();
+    if (t0 == 0) t0 = now;
+    else if (now - t0 > 4000000000ll) return false;
   }
+}
+__device__ __forceinline__ bool tree_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return mbar_try(bar, parity) || tree_wait_long(bar, parity, abort_flag);
+}
+__device__ __noinline__ void tree_give_up(int* status, volatile int* abort_flag, int code) {
+  atomicCAS(status, 0, code);
+  *abort_flag = 1;
 }
 __device__ __forceinline__ float tree_ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// four int8 codes (as x + 128 in a word) -> two words of bf16, exact
+// Four int8 codes -> four bf16, exact: 128 + (x & 127) is 0x4300 | (x & 127) as bf16, and 128 or (x < 0) 256 is 0x4300 | (x & 128).
 __device__ __forceinline__ uint2 codes_to_bf16(uint32_t w) {
-  float f[4];
+  uint2 v;
+  uint32_t* o = &v.x;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) f[i] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650 + i)) - 8388736.f;
-  return make_uint2(pack_bf162(f[0], f[1]), pack_bf162(f[2], f[3]));
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t h = __byte_perm(w, 0, i ? 0x4342 : 0x4140);
+    const uint32_t m = (h & 0x007f007fu) | 0x43004300u, c = (h & 0x00800080u) | 0x43004300u;
+    const bf162 d = __hsub2(*reinterpret_cast<const bf162*>(&m), *reinterpret_cast<const bf162*>(&c));
+    o[i] = *reinterpret_cast<const uint32_t*>(&d);
+  }
+  return v;
 }
 
-// Stages of the rings.  int8: the next page waits in registers, and the scales need room too.
-template <int HD, bool Q8> struct TreeRing { static constexpr int stages = HD == 256 ? (Q8 ? 2 : 3) : HD == 128 ? 4 : 6; };
+// Stages of the rings, and shared memory: rings of K and V, two tiles of P, int8: two pages of codes.  bf16 pages share one ring of
+// twice as many tiles, in the order of their use: the scores of a page are multiplied while the page before is still in the softmax, so
+// K of a page is requested before V of the page before it.  (With a ring each, V tiles wait for their turn where tiles that are needed
+// earlier could be on their way: 2 x 64 nodes behind 65536 tokens XX -> YY us.)
+template <int HD, bool Q8> struct TreeRing {
+  static constexpr int stages = HD == 256 ? (Q8 ? 2 : 3) : HD == 128 ? 4 : 6;
+  static constexpr size_t bytes = (size_t)2 * stages * kPage * HD * 2 + 2 * kRows * kPage * 2 + (Q8 ? (size_t)2 * 2 * kPage * HD : 0);
+};
+
+// Places of page n's tiles in the order of the shared ring, `total` pages in all.
+__device__ __forceinline__ int unit_k(int n) { return n == 0 ? 0 : 2 * n - 1; }
+__device__ __forceinline__ int unit_v(int n, int total) { return n + 1 < total ? 2 * n + 2 : 2 * n + 1; }
 
 template <int HD, bool Q8>
-__global__ void __launch_bounds__(Q8 ? 480 : 352, 1)
+__global__ void __launch_bounds__(Q8 ? 352 + kLoaders : 352, 1)
 tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs a) {
   constexpr int NC = HD / 64, ST = TreeRing<HD, Q8>::stages;
+  // Scales of an int8 page are read until its accumulator is free.  K of page n is converted after the scores of page n - ST, and those
+  // were multiplied after the accumulator of page n - ST - 2 was free.
+  constexpr int SR = ST + 2;
   constexpr int KC = kPage * 128, KV_BYTES = kPage * HD * 2, P_BYTES = kRows * kPage * 2;
   constexpr uint32_t TMEM_COLS = 2 * kPage + HD + HD / 2 <= 256 ? 256 : 512;
   constexpr uint32_t IDESC_S = umma_idesc(kRows, kPage, 1, 1);
   constexpr uint32_t IDESC_O = umma_idesc(kRows, HD, 1, 1) | (1u << 16);     // B operand MN-major
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* Ks = smem_raw;                       // the swizzle wants 1024-byte blocks; there is no room to round up
-  unsigned char* Vs = Ks + ST * KV_BYTES;
-  unsigned char* Ps = Vs + ST * KV_BYTES;             // [2][P_BYTES]
-  __shared__ uint64_t q_full, k_full[ST], v_full[ST], k_free[ST], v_free[ST], s_full[2], s_free[2], p_full[2], p_free[2], o_full, o_free,
-      pair_bar[4];
-  __shared__ float xch[2][2][kRows];                  // [page parity][half][row] maxima
-  __shared__ float lx[kRows];
-  __shared__ float scales[Q8 ? ST : 1][2][kPage];
+  unsigned char* Ps = Ks + 2 * ST * KV_BYTES;         // [2][P_BYTES]
+  unsigned char* Cs = Ps + 2 * P_BYTES;               // int8: [2][K, V codes], each thread's own
+  // bf16: k_full and k_free of all 2 ST places of the shared ring; int8: ST each of K and V
+  __shared__ uint64_t q_full, k_full[2 * ST], k_free[2 * ST], s_full[2], s_free[2], p_full[2], p_free[2], o_full, o_free,
+      m_done[4][2], pair_bar[4], sc_full[Q8 ? SR : 1];
+  __shared__ float mref[kRows];                       // reference maxima
+  __shared__ float scales[Q8 ? SR : 1][2][kPage];     // scale_log2 * key scales, value scales
   __shared__ Segments seg_s;
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
@@ -158,10 +188,14 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     int64_t none, all;
     page_sums(a, 0, &none, &all);
     const int per = a.nkv * a.tiles;
-    const int64_t T = all * per, lo = piece_start(blockIdx.x, T, a.ctas), hi = piece_start(blockIdx.x + 1, T, a.ctas);
+    const int64_t T = all * per;
+    const int G = (int)min((int64_t)a.ctas, T);
+    const bool some = (int)blockIdx.x < G;
+    const int64_t lo = some ? piece_start(blockIdx.x, T, G) : 0, hi = some ? piece_start(blockIdx.x + 1, T, G) : 0;
     int64_t start = 0;
     int r = 0;
     if (lo < hi)                                      // the sequence of the first page: 32 sequences at a time
+#pragma unroll 1
       for (;; r += 32) {
         const int64_t n = r + lane < a.R ? (int64_t)cached_pages(a, r + lane) * per : 0;
         int64_t incl = n;
@@ -180,24 +214,24 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         start += __shfl_sync(0xffffffffu, incl, 31);
       }
     if (lane == 0) {
-      seg_s.g = lo; seg_s.end = hi; seg_s.start = start; seg_s.r = r; seg_s.n = lo < hi ? cached_pages(a, r) : 0;
+      const int n = lo < hi ? cached_pages(a, r) : 1, it = (int)((lo - start) / n);
+      seg_s = Segments{(int)(hi - lo), r, n, it / a.tiles, it % a.tiles, r * per + it, 0, (int)(lo - start) - it * n};
       abort_s = 0;
       mbar_init(&q_full, 8);
       mbar_init(&o_full, 1);
       mbar_init(&o_free, 8);
-      for (int i = 0; i < ST; ++i) {
-        mbar_init(&k_full[i], Q8 ? 128 : 1); mbar_init(&v_full[i], Q8 ? 128 : 1); mbar_init(&k_free[i], 1); mbar_init(&v_free[i], 1);
-      }
+      for (int i = 0; i < 2 * ST; ++i) { mbar_init(&k_full[i], Q8 ? kLoaders / 2 : 1); mbar_init(&k_free[i], 1); }
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 8); mbar_init(&p_full[i], 8); mbar_init(&p_free[i], 1);
+        mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4); mbar_init(&p_free[i], 1);
       }
-      for (int i = 0; i < 4; ++i) mbar_init(&pair_bar[i], 64);
+      for (int i = 0; Q8 && i < SR; ++i) mbar_init(&sc_full[i], 2 * kPage);
+      for (int i = 0; i < 4; ++i) { mbar_init(&m_done[i][0], 1); mbar_init(&m_done[i][1], 1); mbar_init(&pair_bar[i], 64); }
       mbar_fence_init();
     }
   }
   __syncthreads();
   Segments seg = seg_s;
-  if (seg.g >= seg.end) return;                       // no page for this CTA
+  if (seg.left <= 0) return;                          // no page for this CTA
   if (warp == 1) {
     tmem_alloc(&tmem_base_s, TMEM_COLS);
     tmem_relinquish();
@@ -206,30 +240,39 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_s, tmem_o = tmem_base + 2 * kPage, tmem_q = tmem_o + HD;       // S0 | S1 | O | Q
-  auto give_up = [&](int code) { atomicCAS(a.status, 0, code); abort_s = 1; };
+  auto give_up = [&](int code) { tree_give_up(a.status, abort_flag, code); };
+  // tile, barriers and phase of page n
+  const int total = seg.left;
+  auto k_at = [&](int n) { return Q8 ? n % ST : unit_k(n) % (2 * ST); };
+  auto v_at = [&](int n) { return Q8 ? ST + n % ST : unit_v(n, total) % (2 * ST); };
+  auto k_ph = [&](int n) { return (uint32_t)((Q8 ? n / ST : unit_k(n) / (2 * ST)) & 1); };
+  auto v_ph = [&](int n) { return (uint32_t)((Q8 ? n / ST : unit_v(n, total) / (2 * ST)) & 1); };
 
   if (warp == 0) {
     // ------------------------------------ TMA producer ------------------------------------------
     if (!Q8 && lane == 0) {
-      int n = 0;
-      while (seg.next(a) && !*abort_flag)
-        for (int p = seg.p0; p < seg.p1; ++p, ++n) {
-          const int s = n % ST;
-          const uint32_t ph = (n / ST) & 1;
-          const int64_t slot0 = page_slot(a, seg.r, p);
-          if (!tree_wait(&k_free[s], ph ^ 1, abort_flag)) { give_up(90); break; }
-          if (slot0 < 0) mbar_arrive(&k_full[s]);     // no such page: its scores are masked, its values cleared
-          else {
-            mbar_expect_tx(&k_full[s], KV_BYTES);
-            for (int c = 0; c < NC; ++c) tma_load_2d(Ks + s * KV_BYTES + c * KC, &tmK, &k_full[s], seg.kvh * HD + c * 64, (int)slot0);
-          }
-          if (!tree_wait(&v_free[s], ph ^ 1, abort_flag)) { give_up(91); break; }
-          if (slot0 < 0) mbar_arrive(&v_full[s]);
-          else {
-            mbar_expect_tx(&v_full[s], KV_BYTES);
-            for (int c = 0; c < NC; ++c) tma_load_2d(Vs + s * KV_BYTES + c * KC, &tmV, &v_full[s], seg.kvh * HD + c * 64, (int)slot0);
-          }
+      // K of page n, then V of page n - 1
+      Segments vs = seg;
+      int vp = 0, n = 0;
+      bool ok = true, have = false;
+      auto load = [&](const CUtensorMap* map, const Segments& g, int page, int u) {
+        const int64_t slot0 = page_slot(a, g.r, page);
+        if (!tree_wait(&k_free[u % (2 * ST)], (u / (2 * ST) & 1) ^ 1, abort_flag)) { give_up(90); return false; }
+        uint64_t* full = &k_full[u % (2 * ST)];
+        if (slot0 < 0) mbar_arrive(full);             // no such page: its scores are masked, its values cleared
+        else {
+          mbar_expect_tx(full, KV_BYTES);
+          for (int c = 0; c < NC; ++c) tma_load_2d(Ks + (u % (2 * ST)) * KV_BYTES + c * KC, map, full, g.kvh * HD + c * 64, (int)slot0);
         }
+        return true;
+      };
+      auto load_v = [&](int i) {
+        if (!have || vp == vs.p1) { have = vs.next(a); vp = vs.p0; }
+        return load(&tmV, vs, vp++, unit_v(i, total));
+      };
+      while (ok && seg.next(a))
+        for (int p = seg.p0; ok && p < seg.p1; ++p, ++n) ok = load(&tmK, seg, p, unit_k(n)) && (n == 0 || load_v(n - 1));
+      if (ok) load_v(n - 1);
     }
   } else if (warp == 1) {
     // ------------------------------------ S = Q K^T ----------------------------------------------
@@ -240,8 +283,8 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!tree_wait(&q_full, sg & 1, abort_flag)) { give_up(92); break; }
         tc_fence_after();
         for (int p = seg.p0; p < seg.p1; ++p, ++n) {
-          const int s = n % ST, sb = n & 1;
-          if (!tree_wait(&k_full[s], (n / ST) & 1, abort_flag) || !tree_wait(&s_free[sb], ((n >> 1) & 1) ^ 1, abort_flag)) { give_up(93); ok = false; break; }
+          const int s = k_at(n), sb = n & 1;
+          if (!tree_wait(&k_full[s], k_ph(n), abort_flag) || !tree_wait(&s_free[sb], ((n >> 1) & 1) ^ 1, abort_flag)) { give_up(93); ok = false; break; }
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
@@ -262,14 +305,14 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       for (int sg = 0; ok && seg.next(a); ++sg) {
         if (!tree_wait(&o_free, (sg & 1) ^ 1, abort_flag)) { give_up(94); break; }
         for (int p = seg.p0; p < seg.p1; ++p, ++n) {
-          const int s = n % ST, sb = n & 1;
-          if (!tree_wait(&p_full[sb], (n >> 1) & 1, abort_flag) || !tree_wait(&v_full[s], (n / ST) & 1, abort_flag)) { give_up(95); ok = false; break; }
+          const int s = v_at(n), sb = n & 1;
+          if (!tree_wait(&p_full[sb], (n >> 1) & 1, abort_flag) || !tree_wait(&k_full[s], v_ph(n), abort_flag)) { give_up(95); ok = false; break; }
           tc_fence_after();
           const uint64_t pd = umma_desc_sw128(Ps + sb * P_BYTES);
-          const uint64_t vd = umma_desc_mn_sw128(Vs + s * KV_BYTES, KC);
+          const uint64_t vd = umma_desc_mn_sw128(Ks + s * KV_BYTES, KC);
 #pragma unroll
           for (int k = 0; k < 4; ++k) umma_f16(tmem_o, pd + 2 * k, vd + (uint64_t)(k * 16 * 128 >> 4), IDESC_O, p != seg.p0 || k != 0);
-          umma_commit(&v_free[s]);
+          umma_commit(&k_free[s]);
           umma_commit(&p_free[sb]);
         }
         if (ok) umma_commit(&o_full);
@@ -277,209 +320,256 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
   } else if (Q8 && warp >= 11) {
     // ------------------------------------ int8 pages ---------------------------------------------
-    // A thread holds 16 codes of each of kPage * HD / 16 / 128 places of K and of V; the next page's are requested before this one's
-    // are converted.
-    constexpr int PER = kPage * HD / 16 / 128;
-    const int t = threadIdx.x - 352;
-    uint4 kq[PER], vq[PER];
-    float ksc = 0.f, vsc = 0.f;
+    // Half of the loaders take the keys, half the values, each at its own pace.  16 codes of a row are a piece; a quarter warp takes four
+    // pieces of each of two rows, so that its bf16 stores hit all banks once.  (Loops are kept short: with every copy unrolled the code
+    // of all roles leaves the instruction cache, and a page takes twice as long.)
+    constexpr int NT = kLoaders / 2, PER = kPage * HD / 16 / NT, G4 = HD / 64, CODES = kPage * HD, STEP = NT / 4 / G4;
+    const int v = (threadIdx.x - 352) / NT, t = (threadIdx.x - 352) % NT;
+    const int row0 = t / 8 / G4 * 2 + t % 8 / 4, c0 = t / 8 % G4 * 4 + t % 4;          // piece i: row0 + i * STEP, c0
+    const int8_t* pool = (const int8_t*)(v ? a.vpool : a.kpool);
+    const float* pscale = v ? a.vscale : a.kscale;
+    const float smul = v ? 1.f : a.scale_log2;
+    const int64_t pitch = (int64_t)a.nkv * HD;
+    unsigned char* const mine = Cs + v * 2 * CODES + t * 16;                            // two pages of this thread's own pieces
+    unsigned char* const to0 = Ks + v * ST * KV_BYTES + (c0 / 4) * KC + row0 * 128;
+    const int piece = (c0 % 4) * 2, at0 = (piece ^ (row0 & 7)) << 4, at1 = ((piece + 1) ^ (row0 & 7)) << 4;      // STEP is a multiple of 8
+    float s0 = 0.f, s1 = 0.f;                         // scale of row t of the page to convert and of the one after it
     Segments ahead = seg;
     int ap = 0;
-    bool have = false;
-    auto fetch = [&]() {                              // the page after the last one fetched
-      if (!have || ap >= ahead.p1) {
-        if (!ahead.next(a)) { have = false; return; }
-        ap = ahead.p0;
-        have = true;
-      }
-      const int64_t slot0 = page_slot(a, ahead.r, ap);
-      const int valid = slot0 < 0 ? 0 : min(kPage, cached_keys(a, ahead.r) - ap * kPage);
-#pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int idx = i * 128 + t, row = idx / (HD / 16), c = idx % (HD / 16);
-        kq[i] = vq[i] = make_uint4(0, 0, 0, 0);
-        if (row < valid) {
-          const int64_t at = ((slot0 + row) * a.nkv + ahead.kvh) * HD + c * 16;
-          kq[i] = ld_stream((const int8_t*)a.kpool + at);
-          vq[i] = ld_stream((const int8_t*)a.vpool + at);
+#pragma unroll 1
+    for (int n = -2; n < total; ++n) {
+      if (n >= 0) {
+        const int st = n % ST;
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (!tree_wait(&k_free[v * ST + st], (n / ST & 1) ^ 1, abort_flag)) { if (lane == 0) give_up(96); break; }
+        if (t < kPage) {
+          scales[Q8 ? n % SR : 0][v][t] = s0 * smul;
+          mbar_arrive(&sc_full[Q8 ? n % SR : 0]);
         }
-      }
-      if (t < kPage) {
-        const int64_t row = (slot0 + t) * a.nkv + ahead.kvh;
-        ksc = t < valid ? a.kscale[row] : 0.f;
-        vsc = t < valid ? a.vscale[row] : 0.f;
-      }
-      ++ap;
-    };
-    auto store = [&](unsigned char* to, const uint4* q) {
+        const unsigned char* codes = mine + (n & 1) * CODES;
+        unsigned char* to = to0 + st * KV_BYTES;
 #pragma unroll
-      for (int i = 0; i < PER; ++i) {
-        const int idx = i * 128 + t, row = idx / (HD / 16), c = idx % (HD / 16);
-        unsigned char* at = to + (c / 4) * KC + row * 128;
-        const int piece = (c % 4) * 2;
-        const uint2 x = codes_to_bf16(q[i].x ^ 0x80808080u), y = codes_to_bf16(q[i].y ^ 0x80808080u);
-        const uint2 z = codes_to_bf16(q[i].z ^ 0x80808080u), w = codes_to_bf16(q[i].w ^ 0x80808080u);
-        *reinterpret_cast<uint4*>(at + ((piece ^ (row & 7)) << 4)) = make_uint4(x.x, x.y, y.x, y.y);
-        *reinterpret_cast<uint4*>(at + (((piece + 1) ^ (row & 7)) << 4)) = make_uint4(z.x, z.y, w.x, w.y);
-      }
-    };
-    fetch();
-    int n = 0;
-    bool ok = true;
-    while (ok && seg.next(a))
-      for (int p = seg.p0; p < seg.p1; ++p, ++n) {
-        const int s = n % ST;
-        const uint32_t ph = (n / ST) & 1;
-        // both products of the stage's last page are done, so nobody reads its scales either
-        if (!tree_wait(&k_free[s], ph ^ 1, abort_flag) || !tree_wait(&v_free[s], ph ^ 1, abort_flag)) { if (lane == 0) give_up(96); ok = false; break; }
-        store(Ks + s * KV_BYTES, kq);
-        store(Vs + s * KV_BYTES, vq);
-        if (t < kPage) { scales[Q8 ? s : 0][0][t] = ksc; scales[Q8 ? s : 0][1][t] = vsc; }
+        for (int i = 0; i < PER; ++i) {
+          const uint4 x = *reinterpret_cast<const uint4*>(codes + i * NT * 16);
+          const uint2 x0 = codes_to_bf16(x.x), x1 = codes_to_bf16(x.y), x2 = codes_to_bf16(x.z), x3 = codes_to_bf16(x.w);
+          *reinterpret_cast<uint4*>(to + i * STEP * 128 + at0) = make_uint4(x0.x, x0.y, x1.x, x1.y);
+          *reinterpret_cast<uint4*>(to + i * STEP * 128 + at1) = make_uint4(x2.x, x2.y, x3.x, x3.y);
+        }
         fence_async_smem();
-        mbar_arrive(&k_full[s]);
-        mbar_arrive(&v_full[s]);
-        fetch();
+        mbar_arrive(&k_full[v * ST + st]);
       }
+      // codes of page n + 2, into the place that was just read, by the same threads
+      s0 = s1;
+      if (n + 2 < total) {
+        if (n == -2 || ap == ahead.p1) {
+          ahead.next(a);
+          ap = ahead.p0;
+        }
+        const int64_t slot0 = page_slot(a, ahead.r, ap);
+        const int valid = slot0 < 0 ? 0 : min(kPage, cached_keys(a, ahead.r) - ap * kPage);
+        const uint32_t to = smem_u32(mine + (n & 1) * CODES);
+        const int8_t* from = pool + (valid ? (slot0 + row0) * pitch + ahead.kvh * HD + c0 * 16 : 0);
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const bool in = row0 + i * STEP < valid;    // else zeros, and the address is not read
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * NT * 16), "l"(in ? from + i * STEP * pitch : pool), "r"(in ? 16 : 0));
+        }
+        s1 = t < valid ? pscale[(slot0 + t) * a.nkv + ahead.kvh] : 0.f;
+        ++ap;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp < 10) {
     // ------------------------------------ softmax, sums -------------------------------------------
-    const int q = warp & 3, hf = (warp - 2) >> 2, r = q * 32 + lane;
+    const int q = warp & 3, grp = (warp - 2) >> 2, r = q * 32 + lane;
     const uint32_t lane_base = (uint32_t)(q * 32) << 16;
-    int n = 0;
-    uint32_t xph = 0;
-    bool ok = true;
-    for (int sg = 0; ok && seg.next(a); ++sg) {
-      const int row = seg.tile * kRows + r, rows = a.C * a.rep;
-      const bool idle = seg.tile * kRows + q * 32 >= rows;     // no row in this quadrant: its lanes only keep the barriers going
-      const int keys = cached_keys(a, seg.r);
-      if (!idle) {
-        const int rr = min(row, rows - 1);
-        const bf16* qrow = a.q + (((int64_t)seg.r * a.C + rr / a.rep) * a.nh + seg.kvh * a.rep + rr % a.rep) * HD;
+    const int rows = a.C * a.rep;
+    // This warp's own 4 KB of the P tiles, 32 rows of 128 bytes in 16-byte pieces c at c ^ (row % 8), between segments: rows go to and from
+    // tensor memory a thread each, and to and from global memory eight threads each.
+    unsigned char* const own = Ps + grp * P_BYTES + q * 4096;
+    const int sub = lane >> 3, pc = lane & 7;
+    auto load_q = [&](const Segments& g) {            // 32 rows of the segment's Q into tensor memory, every other 64 columns a group
+      const int first = g.tile * kRows + q * 32;
+      if (first < rows) {
+        const bf16* qs = a.q + ((int64_t)g.r * a.C * a.nh + g.kvh * a.rep) * HD;
 #pragma unroll 1
-        for (int i = hf; i < NC; i += 2) {
-          uint32_t w[32];
+        for (int i = grp; i < NC; i += 2) {
+          uint4 x[8];
 #pragma unroll
           for (int v = 0; v < 8; ++v) {
-            const uint4 x = *reinterpret_cast<const uint4*>(qrow + i * 64 + v * 8);
-            w[4 * v] = x.x; w[4 * v + 1] = x.y; w[4 * v + 2] = x.z; w[4 * v + 3] = x.w;
+            const int rr = min(first + v * 4 + sub, rows - 1);
+            x[v] = *reinterpret_cast<const uint4*>(qs + ((int64_t)(rr / a.rep) * a.nh + rr % a.rep) * HD + i * 64 + pc * 8);
           }
+#pragma unroll
+          for (int v = 0; v < 8; ++v) *reinterpret_cast<uint4*>(own + (v * 4 + sub) * 128 + ((pc ^ ((v * 4 + sub) & 7)) << 4)) = x[v];
+          __syncwarp();
+          uint32_t w[32];
+#pragma unroll
+          for (int v = 0; v < 8; ++v) *reinterpret_cast<uint4*>(w + 4 * v) = *reinterpret_cast<const uint4*>(own + lane * 128 + ((v ^ (lane & 7)) << 4));
           tmem_st32(tmem_q + lane_base + i * 32, w);
+          __syncwarp();
         }
         tmem_st_wait();
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
-      float m_ref = -INFINITY, l = 0.f;
+    };
+    int n = 0;
+    bool ok = true;
+    Segments ahead = seg;
+    bool more = ahead.next(a);
+    if (more) load_q(ahead);
+    for (int sg = 0; ok && more; ++sg) {
+      seg = ahead;
+      const bool idle = seg.tile * kRows + q * 32 >= rows;     // no row in this quadrant: its lanes only keep the barriers going
+      const int keys = cached_keys(a, seg.r), row = seg.tile * kRows + r;
+      float m = -INFINITY, l = 0.f;
       for (int p = seg.p0; p < seg.p1; ++p, ++n) {
-        const int sb = n & 1, s = n % ST;
-        const uint32_t ph = (n >> 1) & 1;
+        const int sb = n & 1, s = n % SR;
+        if (sb != grp) continue;
         const int valid = page_slot(a, seg.r, p) < 0 ? 0 : min(kPage, keys - p * kPage);
-        if (!tree_wait(&s_full[sb], ph, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
-        if (Q8 && !tree_wait(&k_full[s], (n / ST) & 1, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
+        if (!tree_wait(&s_full[sb], (n >> 1) & 1, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
+        if (Q8 && !tree_wait(&sc_full[Q8 ? s : 0], (n / SR) & 1, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
         tc_fence_after();
-        uint32_t sv[32];
-        if (!idle) {
-          tmem_ld32(tmem_base + lane_base + sb * kPage + hf * 32, sv);
+        // scores of columns [32 h, 32 h + 32): scaled, int8; raw, bf16.  They are read twice, for the maximum and for the weights, which
+        // leaves half the registers and half the code of holding them.
+        auto scores = [&](int h, uint32_t* sv) {
+          tmem_ld32(tmem_base + lane_base + sb * kPage + h * 32, sv);
           tmem_ld_wait();
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[sb]);
-        if (!idle) {
-          float mx0 = -INFINITY, mx1 = -INFINITY;
           if (Q8) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) sv[c] = __float_as_uint(__uint_as_float(sv[c]) * (a.scale_log2 * scales[Q8 ? s : 0][0][hf * 32 + c]));
-          } else {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) sv[c] = __float_as_uint(__uint_as_float(sv[c]) * a.scale_log2);
+            for (int c = 0; c < 32; ++c) sv[c] = __float_as_uint(__uint_as_float(sv[c]) * scales[Q8 ? s : 0][0][h * 32 + c]);
           }
           if (valid < kPage) {
 #pragma unroll
             for (int c = 0; c < 32; ++c)
-              if (hf * 32 + c >= valid) sv[c] = __float_as_uint(-INFINITY);
+              if (h * 32 + c >= valid) sv[c] = __float_as_uint(-INFINITY);
           }
-#pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            mx0 = fmaxf(mx0, __uint_as_float(sv[c]));
-            mx1 = fmaxf(mx1, __uint_as_float(sv[c + 1]));
-          }
-          xch[sb][hf][r] = fmaxf(mx0, mx1);
-        }
-        mbar_arrive(&pair_bar[q]);
-        if (!tree_wait(&pair_bar[q], xph, abort_flag)) { if (lane == 0) give_up(98); ok = false; break; }
-        xph ^= 1;
-        uint32_t pk[16];
+        };
+        float mx = -INFINITY;
         if (!idle) {
-          const float mx = fmaxf(xch[sb][0][r], xch[sb][1][r]);
-          if (p == seg.p0) m_ref = mx;
-          else if (__any_sync(0xffffffffu, mx > m_ref + 8.f)) {
-            // every product that wrote O has to be complete; the one of this page cannot start before P
-            if (!tree_wait(&p_free[(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag)) { if (lane == 0) give_up(99); ok = false; break; }
-            tc_fence_after();
-            const float m_new = fmaxf(m_ref, mx), f = m_new == -INFINITY ? 1.f : tree_ex2(m_ref - m_new);
-            m_ref = m_new;
-            l *= f;
+          float mx1 = -INFINITY;
 #pragma unroll 1
-            for (int c0 = hf * (HD / 2); c0 < (hf + 1) * (HD / 2); c0 += 32) {
-              uint32_t o[32];
-              tmem_ld32(tmem_o + lane_base + c0, o);
-              tmem_ld_wait();
+          for (int h = 0; h < 2; ++h) {
+            uint32_t sv[32];
+            scores(h, sv);
 #pragma unroll
-              for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-              tmem_st32(tmem_o + lane_base + c0, o);
+            for (int c = 0; c < 32; c += 2) {
+              mx = fmaxf(mx, __uint_as_float(sv[c]));
+              mx1 = fmaxf(mx1, __uint_as_float(sv[c + 1]));
             }
-            tmem_st_wait();
-            tc_fence_before();
           }
-          const float ms = m_ref == -INFINITY ? 0.f : m_ref;
-          float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            float p0 = tree_ex2(__uint_as_float(sv[2 * c]) - ms), p1 = tree_ex2(__uint_as_float(sv[2 * c + 1]) - ms);
-            l0 += p0; l1 += p1;
-            if (Q8) { p0 *= scales[Q8 ? s : 0][1][hf * 32 + 2 * c]; p1 *= scales[Q8 ? s : 0][1][hf * 32 + 2 * c + 1]; }
-            pk[c] = pack_bf162(p0, p1);               // weights rounded to bf16, half a step 2^-8; their sum is not
-          }
-          l += l0 + l1;
+          mx = fmaxf(mx, mx1);
+          if (!Q8) mx *= a.scale_log2;
         }
+        if (p == seg.p0) m = mx;
+        else {                                        // the other group has left the reference of the page before
+          if (!tree_wait(&m_done[q][sb ^ 1], ((n - 1) >> 1) & 1, abort_flag)) { if (lane == 0) give_up(98); ok = false; break; }
+          if (!idle) {
+            const float was = mref[r];
+            if (was != m) {
+              l = l > 0.f ? l * tree_ex2(m - was) : l;
+              m = was;
+            }
+            if (__any_sync(0xffffffffu, mx > m + 8.f)) {
+              // every product that wrote O has to be complete; the one of this page cannot start before P
+              if (!tree_wait(&p_free[sb ^ 1], ((n - 1) >> 1) & 1, abort_flag)) { if (lane == 0) give_up(99); ok = false; break; }
+              tc_fence_after();
+              const float m_new = fmaxf(m, mx), f = m_new == -INFINITY ? 1.f : tree_ex2(m - m_new);
+              m = m_new;
+              l *= f;
+#pragma unroll 1
+              for (int c0 = 0; c0 < HD; c0 += 32) {
+                uint32_t o[32];
+                tmem_ld32(tmem_o + lane_base + c0, o);
+                tmem_ld_wait();
+#pragma unroll
+                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                tmem_st32(tmem_o + lane_base + c0, o);
+              }
+              tmem_st_wait();
+              tc_fence_before();
+            }
+          }
+        }
+        if (!idle) mref[r] = m;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m_done[q][sb]);
+        const float ms = m == -INFINITY ? 0.f : m;
         if (n >= 2 && !tree_wait(&p_free[sb], ((n - 2) >> 1) & 1, abort_flag)) { if (lane == 0) give_up(100); ok = false; break; }
         if (!idle) {
           unsigned char* prow = Ps + sb * P_BYTES + r * 128;
+          float l0 = 0.f, l1 = 0.f;
+#pragma unroll 1
+          for (int h = 0; h < 2; ++h) {
+            uint32_t sv[32];
+            scores(h, sv);
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            *reinterpret_cast<uint4*>(prow + (((hf * 4 + c) ^ (r & 7)) << 4)) = make_uint4(pk[4 * c], pk[4 * c + 1], pk[4 * c + 2], pk[4 * c + 3]);
+            for (int c = 0; c < 4; ++c) {
+              uint32_t pk[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int k = c * 8 + i * 2;
+                float p0 = __uint_as_float(sv[k]), p1 = __uint_as_float(sv[k + 1]);
+                p0 = tree_ex2(Q8 ? p0 - ms : fmaf(p0, a.scale_log2, -ms));
+                p1 = tree_ex2(Q8 ? p1 - ms : fmaf(p1, a.scale_log2, -ms));
+                l0 += p0; l1 += p1;
+                if (Q8) { p0 *= scales[Q8 ? s : 0][1][h * 32 + k]; p1 *= scales[Q8 ? s : 0][1][h * 32 + k + 1]; }
+                pk[i] = pack_bf162(p0, p1);           // weights rounded to bf16, half a step 2^-8; their sum is not
+              }
+              *reinterpret_cast<uint4*>(prow + (((h * 4 + c) ^ (r & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+            }
+          }
+          l += l0 + l1;
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[sb]);      // the accumulator may take S of page n + 2
         if (!Q8 && valid < kPage) {                   // 0 times what lies behind the cache is not always 0: clear it
-          if (!tree_wait(&v_full[s], (n / ST) & 1, abort_flag)) { if (lane == 0) give_up(101); ok = false; break; }
+          if (!tree_wait(&k_full[v_at(n)], v_ph(n), abort_flag)) { if (lane == 0) give_up(101); ok = false; break; }
           const int per = (kPage - valid) * 8;        // 16-byte pieces of a chunk
-          for (int i = (warp - 2) * 32 + lane; i < NC * per; i += 256)
-            *reinterpret_cast<uint4*>(Vs + s * KV_BYTES + (i / per) * KC + valid * 128 + (i % per) * 16) = make_uint4(0, 0, 0, 0);
+          for (int i = q * 32 + lane; i < NC * per; i += 128)
+            *reinterpret_cast<uint4*>(Ks + v_at(n) * KV_BYTES + (i / per) * KC + valid * 128 + (i % per) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[sb]);
       }
       if (!ok) break;
-      if (!tree_wait(&o_full, sg & 1, abort_flag)) { if (lane == 0) give_up(102); break; }
+      if (!tree_wait(&o_full, sg & 1, abort_flag) || !tree_wait(&m_done[q][(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag)) { if (lane == 0) give_up(102); break; }
       tc_fence_after();
-      if (hf == 1) lx[r] = l;
+      // all products of the segment are done: Q, O and the P tiles are free
+      more = ahead.next(a);
+      if (more) load_q(ahead);
+      const float was = idle ? 0.f : mref[r];
+      l = l > 0.f ? l * tree_ex2(m - was) : l;
       mbar_arrive(&pair_bar[q]);
-      if (!tree_wait(&pair_bar[q], xph, abort_flag)) { if (lane == 0) give_up(103); break; }
-      xph ^= 1;
+      if (!tree_wait(&pair_bar[q], 0, abort_flag)) { if (lane == 0) give_up(103); break; }
+      // the odd group's sums by way of the even group's tile, which nobody else writes
+      if (grp == 1) reinterpret_cast<float*>(own - P_BYTES)[lane] = l;
+      mbar_arrive(&pair_bar[q]);
+      if (!tree_wait(&pair_bar[q], 1, abort_flag)) { if (lane == 0) give_up(103); break; }
       if (!idle) {
-        const int64_t at = ((int64_t)blockIdx.x + seg.item) * a.used + r;
-        if (hf == 0 && row < rows) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_ref, l + lx[r]);
+        const int64_t at = ((int64_t)blockIdx.x + seg.item) * a.used + q * 32;         // the warp's first row
+        if (grp == 0 && row < rows) *reinterpret_cast<float2*>(a.part_ml + (at + lane) * 2) = make_float2(was, l + reinterpret_cast<const float*>(own)[lane]);
+        __syncwarp();
+        const int here = min(32, rows - seg.tile * kRows - q * 32);
 #pragma unroll 1
-        for (int c0 = hf * (HD / 2); c0 < (hf + 1) * (HD / 2); c0 += 32) {
+        for (int c0 = grp * (HD / 2); c0 < (grp + 1) * (HD / 2); c0 += 32) {
           uint32_t o[32];
           tmem_ld32(tmem_o + lane_base + c0, o);
           tmem_ld_wait();
-          if (row < rows) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
-              *reinterpret_cast<uint4*>(a.part_o + at * HD + c0 + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+          for (int v = 0; v < 8; ++v) *reinterpret_cast<uint4*>(own + lane * 128 + ((v ^ (lane & 7)) << 4)) = *reinterpret_cast<const uint4*>(o + 4 * v);
+          __syncwarp();
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            const int rr = v * 4 + sub;
+            if (rr < here) *reinterpret_cast<uint4*>(a.part_o + (at + rr) * HD + c0 + pc * 4) = *reinterpret_cast<const uint4*>(own + rr * 128 + ((pc ^ (rr & 7)) << 4));
           }
+          __syncwarp();
         }
       }
       tc_fence_before();
@@ -491,8 +581,8 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   tc_fence_before();
   __syncthreads();
   if (abort_s) {                                      // copies still in flight land before the shared memory is released
-    const uint64_t t0 = tree_now();
-    while (tree_now() - t0 < 2000000ull) __nanosleep(1000);
+    const long long t0 = clock64();
+    while (clock64() - t0 < 4000000ll) __nanosleep(1000);
   }
   if (warp == 1) {
     tc_fence_after();
@@ -500,7 +590,35 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   }
 }
 
-// A warp a (node, head): the node's path, then the partial sums of the cache, the gate and the store.  Lanes own hd / 32 channels.
+// EPL channels of one lane of a pool row, as floats (codes unscaled)
+template <int EPL, bool Q8>
+__device__ __forceinline__ void row_piece(const void* pool, int64_t at, float* x) {
+  if (Q8) {
+    const int8_t* p = (const int8_t*)pool + at;
+    if (EPL == 8) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) x[e] = (float)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)) & 0xff);
+    } else {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) x[e] = (float)p[e];
+    }
+  } else {
+    const bf16* p = (const bf16*)pool + at;
+    if (EPL == 8) bf16x8_to_float(*reinterpret_cast<const uint4*>(p), x);
+    else {
+#pragma unroll
+      for (int e = 0; e < EPL; e += 2) {
+        const float2 f = __bfloat1622float2(*reinterpret_cast<const bf162*>(p + e));
+        x[e] = f.x; x[e + 1] = f.y;
+      }
+    }
+  }
+}
+
+// A warp a (node, head): the node's path, the partial sums of the cache, the gate and the store.  Lanes own hd / 32 channels of a row;
+// lane i also keeps slot and score of nodes i and i + 32, and the maximum and sum of a partial.  Latency is all there is to it: tables,
+// scores and maxima are fetched by all lanes at once, rows four at a time.
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) {
   constexpr int EPL = HD / 32;
@@ -516,60 +634,136 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
   on = (on & (~0ull >> (63 - j))) | 1ull << j;              // a path ends at its node
   const int kvh = h / a.rep;
   const int64_t row = (int64_t)r * a.C + j;
-  float q[EPL], o[EPL], m = -INFINITY, l = 0.f;
+  float q[EPL], o[EPL], gate[EPL];
+  row_piece<EPL, false>(a.q, (row * a.nh + h) * HD + lane * EPL, q);
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) {
-    q[e] = __bfloat162float(a.q[(row * a.nh + h) * HD + lane * EPL + e]) * a.scale_log2;
-    o[e] = 0.f;
+  for (int e = 0; e < EPL; ++e) { q[e] *= a.scale_log2; o[e] = 0.f; gate[e] = 0.f; }
+  if (a.gate) row_piece<EPL, false>(a.gate, row * a.ldg + (int64_t)h * 2 * HD + HD + lane * EPL, gate);
+  // pool rows of the path; a page that is none takes its nodes off it
+  int64_t kr[2];
+  float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f}, sc[2] = {-INFINITY, -INFINITY};
+  uint64_t path = 0;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int i = lane + 32 * u, p = pos0 + i;
+    const bool mine = on >> i & 1;
+    const int64_t slot0 = mine ? page_slot(a, r, p / kPage) : -1;
+    kr[u] = slot0 < 0 ? 0 : (slot0 + p % kPage) * a.nkv + kvh;
+    if (Q8 && slot0 >= 0) { ks[u] = a.kscale[kr[u]]; vs[u] = a.vscale[kr[u]]; }
+    path |= (uint64_t)__ballot_sync(0xffffffffu, slot0 >= 0) << (32 * u);
   }
-  while (on) {
-    const int i = __ffsll((long long)on) - 1;
-    on &= on - 1;
-    const int p = pos0 + i;
-    const int64_t slot0 = page_slot(a, r, p / kPage);
-    if (slot0 < 0) continue;
-    const int64_t kr = (slot0 + p % kPage) * a.nkv + kvh;
-    float k[EPL], v[EPL];
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) {
-      const int64_t at = kr * HD + lane * EPL + e;
-      k[e] = Q8 ? (float)((const int8_t*)a.kpool)[at] * a.kscale[kr] : __bfloat162float(((const bf16*)a.kpool)[at]);
-      v[e] = Q8 ? (float)((const int8_t*)a.vpool)[at] * a.vscale[kr] : __bfloat162float(((const bf16*)a.vpool)[at]);
-    }
-    float s = 0.f;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) s = fmaf(q[e], k[e], s);
-    s = warp_sum(s);
-    const float mn = fmaxf(m, s), ms = mn == -INFINITY ? 0.f : mn, c = exp2f(m - ms), w = exp2f(s - ms);
-    m = mn;
-    l = l * c + w;
-#pragma unroll
-    for (int e = 0; e < EPL; ++e) o[e] = o[e] * c + w * v[e];
-  }
+  // the cache's partials: maxima and sums, one a lane
   int64_t before, all;
   page_sums(a, r, &before, &all);
-  const int n = cached_pages(a, r);
+  const int n = cached_pages(a, r), per = a.nkv * a.tiles, lrow = j * a.rep + h % a.rep, it = kvh * a.tiles + lrow / kRows, item = r * per + it;
+  int b0 = 0, parts = 0;
   if (n > 0) {
-    const int per = a.nkv * a.tiles, lrow = j * a.rep + h % a.rep, it = kvh * a.tiles + lrow / kRows, item = r * per + it;
     const int64_t T = all * per, g0 = before * per + (int64_t)it * n;
-    const int b0 = piece_of(g0, T, a.ctas), b1 = piece_of(g0 + n - 1, T, a.ctas);
-    for (int b = b0; b <= b1; ++b) {
-      const int64_t at = (int64_t)(b + item) * a.used + lrow % kRows;
-      if (piece_start(b, T, a.ctas) == piece_start(b + 1, T, a.ctas)) continue;      // fewer pages than pieces: an empty one
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + at * 2);
-      if (ml.x == -INFINITY) continue;                      // no key in these pages
-      const float mn = fmaxf(m, ml.x), c = exp2f(m - mn), w = exp2f(ml.x - mn);
-      m = mn;
-      l = l * c + ml.y * w;
+    const int G = (int)min((int64_t)a.ctas, T);
+    b0 = piece_of(g0, T, G);
+    parts = piece_of(g0 + n - 1, T, G) - b0 + 1;
+  }
+  float m = -INFINITY;
+#pragma unroll 1
+  for (int b = lane; b < parts; b += 32) m = fmaxf(m, a.part_ml[((int64_t)(b0 + b + item) * a.used + lrow % kRows) * 2]);
+  // scores of the path
+  auto take = [&](uint64_t& rest) {                         // next node, -1: none left
+    const int i = rest ? __ffsll((long long)rest) - 1 : -1;
+    rest &= rest - 1;
+    return i;
+  };
+#pragma unroll 1
+  for (uint64_t rest = path; rest;) {
+    int id[4];
+    float s[4];
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) o[e] = o[e] * c + w * a.part_o[at * HD + lane * EPL + e];
+    for (int k = 0; k < 4; ++k) {
+      id[k] = take(rest);
+      const int64_t at = id[k] < 32 ? __shfl_sync(0xffffffffu, kr[0], id[k] & 31) : __shfl_sync(0xffffffffu, kr[1], id[k] & 31);
+      float x[EPL];
+      s[k] = 0.f;
+      if (id[k] >= 0) {
+        row_piece<EPL, Q8>(a.kpool, at * HD + lane * EPL, x);
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) s[k] = fmaf(q[e], x[e], s[k]);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      s[k] = warp_sum(s[k]);
+      if (id[k] == lane) sc[0] = s[k] * ks[0];
+      if (id[k] == lane + 32) sc[1] = s[k] * ks[1];
     }
   }
+  m = warp_max(fmaxf(m, fmaxf(sc[0], sc[1])));
+  const float ms = m == -INFINITY ? 0.f : m;
+  float w[2] = {exp2f(sc[0] - ms), exp2f(sc[1] - ms)}, l = w[0] + w[1];
+  w[0] *= vs[0]; w[1] *= vs[1];
+#pragma unroll 1
+  for (uint64_t rest = path; rest;) {
+    float x[4][EPL], f[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = take(rest);
+      const int64_t at = i < 32 ? __shfl_sync(0xffffffffu, kr[0], i & 31) : __shfl_sync(0xffffffffu, kr[1], i & 31);
+      f[k] = i < 32 ? __shfl_sync(0xffffffffu, w[0], i & 31) : __shfl_sync(0xffffffffu, w[1], i & 31);
+      if (i >= 0) row_piece<EPL, Q8>(a.vpool, at * HD + lane * EPL, x[k]);
+      else {
+        f[k] = 0.f;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) x[k][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[e] = fmaf(f[k], x[k][e], o[e]);
+  }
+#pragma unroll 1
+  for (int c = 0; c < parts; c += 32) {
+    float f = 0.f;
+    if (c + lane < parts) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + ((int64_t)(b0 + c + lane + item) * a.used + lrow % kRows) * 2);
+      f = exp2f(ml.x - ms);                                 // 0 where these pages hold no key
+      l += f * ml.y;
+    }
+    const int here = min(32, parts - c);
+#pragma unroll 1
+    for (int b = 0; b < here; b += 4) {
+      float x[4][EPL], g[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        g[k] = __shfl_sync(0xffffffffu, f, (b + k) & 31);
+        const bool in = b + k < here;
+        const float* po = a.part_o + ((int64_t)(b0 + c + b + k + item) * a.used + lrow % kRows) * HD + lane * EPL;
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) x[k][e] = 0.f;
+        if (in) {
+          if (EPL == 8) {
+            *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(po);
+            *reinterpret_cast<float4*>(x[k] + EPL / 2) = *reinterpret_cast<const float4*>(po + 4);
+          } else {
+#pragma unroll
+            for (int e = 0; e < EPL; ++e) x[k][e] = po[e];
+          }
+        } else g[k] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+#pragma unroll
+        for (int e = 0; e < EPL; ++e) o[e] = fmaf(g[k], x[k][e], o[e]);
+    }
+  }
+  l = warp_sum(l);
   const float inv = l > 0.f ? 1.f / l : 0.f;
-  const bf16* gp = a.gate ? a.gate + row * a.ldg + (int64_t)h * 2 * HD + HD + lane * EPL : nullptr;
   bf16* op = a.out + row * a.ldo + (int64_t)h * HD + lane * EPL;
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) op[e] = __float2bfloat16(o[e] * inv * (gp ? sigmoid_f(__bfloat162float(gp[e])) : 1.f));
+  for (int e = 0; e < EPL; ++e) o[e] *= inv * (a.gate ? sigmoid_f(gate[e]) : 1.f);
+  if (EPL == 8) *reinterpret_cast<uint4*>(op) = float_to_bf16x8(o);
+  else {
+#pragma unroll
+    for (int e = 0; e < EPL; e += 2) *reinterpret_cast<uint32_t*>(op + e) = pack_bf162(o[e], o[e + 1]);
+  }
 }
 
 template <int HD, bool Q8>
@@ -580,11 +774,11 @@ int launch_tree(const TreeAttnArgs& a, int64_t slots, cudaStream_t st) {
     if (!rc) rc = cb_make_tmap_2d(&tmV, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.vpool, (uint64_t)slots, (uint64_t)a.nkv * HD, (uint64_t)a.nkv * HD, kPage, 64);
     if (rc) return rc;
   }
-  const size_t smem = (size_t)2 * TreeRing<HD, Q8>::stages * kPage * HD * 2 + 2 * kRows * kPage * 2;
+  const size_t smem = TreeRing<HD, Q8>::bytes;
   auto kern = tree_cache_kernel<HD, Q8>;
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
-  e = cb_launch(kern, dim3((unsigned)a.ctas), dim3(Q8 ? 480 : 352), smem, st, tmK, tmV, a);
+  e = cb_launch(kern, dim3((unsigned)a.ctas), dim3(Q8 ? 352 + kLoaders : 352), smem, st, tmK, tmV, a);
   if (e != cudaSuccess) return (int)e;
   const int64_t tasks = (int64_t)a.R * a.C * a.nh;
   return (int)cb_launch(tree_finish_kernel<HD, Q8>, dim3((unsigned)((tasks + 7) / 8)), dim3(256), 0, st, a);
@@ -599,7 +793,7 @@ CB_EXPORT int cb_attn_tree(const void* q, const void* gate, int64_t ldg, const v
                            int64_t hd, void* status, void* stream) {
   if (!q || !kpool || !vpool || !tables || !positions || !anc || !out || !part || !status) return CB_ERR_ARG;
   if ((kscale == nullptr) != (vscale == nullptr)) return CB_ERR_ARG;
-  if (R < 1 || C < 1 || C > kMaxNodes || nkv < 1 || nh % nkv || ctas < 1 || ctas > 65535 || width < 1 || width > (1 << 24) || R * C * nh > (1ll << 30) || slots > 0x7fffffff ||
+  if (R < 1 || C < 1 || C > kMaxNodes || nkv < 1 || nh % nkv || ctas < 1 || ctas > 65535 || width < 1 || width > (1 << 24) || R * C * nh > (1ll << 30) || R * width * nkv * ((C * (nh / nkv) + kRows - 1) / kRows) > 0x7fffffff || slots > 0x7fffffff ||
       ((uintptr_t)part & 15)) return CB_ERR_SHAPE;
   const int64_t rows = C * (nh / nkv), tiles = (rows + kRows - 1) / kRows, used = rows < kRows ? rows : kRows;
   const int64_t places = (ctas + R * nkv * tiles) * used;

@@ -65,6 +65,8 @@ class Attn:
                               hd=self.hd, kscale=self.kscale, vscale=self.vscale)
 
     def check(self, out=None):
+        from coffin_b200.ops import kernels as K
+        K.check_status()                                   # no bounded wait ran out
         R, C, nh, hd = self.R, self.C, self.nh, self.hd
         gate = self.proj[:, :nh * 2 * hd].reshape(R, C, nh, 2, hd)[:, :, :, 1] if self.proj is not None else None
         ref, bound = P.attn(self.q.view(R, C, nh, hd), gate, self.kpool, self.vpool, self.kscale, self.vscale, self.tables.tolist(), self.contexts,
