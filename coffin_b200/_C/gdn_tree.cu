@@ -8,9 +8,15 @@
 // convolution along the path: its older taps are the node's ancestors, behind them the ring.  State and ring stay as they were; k, d and
 // alpha of every node are recorded and the raw rows kept, from which a commit replays the accepted path (tree_commit.cu).
 //
-// A CTA owns DVS columns of one head's state (columns are independent but for the norm, whose sums of squares the CTAs of a cluster
-// exchange).  Everything is fp32; sums of g along a path are 64-bit, since differences of them are exponents.  Entries of the Gram
-// matrices off a node's path are never multiplied, so a node's values do not reach its siblings whatever they are.
+// 1. rows: a warp a (node, head) convolves, norms q and k and leaves them, and v, as fp32 rows by head.  (Within the kernel below it was
+//    repeated for every value head of a key head and every group of columns.)
+// 2. nodes: a CTA owns DVS columns of one head's state; the DV / DVS CTAs of a head are a cluster, share out the Gram matrices and
+//    exchange the sums of squares of the norm.  (1 - A)^-1 of the strictly lower matrix A of the first equation is built from inverted 8 x 8
+//    blocks by doubling, so that what follows are small dense products.
+// Everything is fp32, as the recorded updates are; the products with the state are most of it (2 C DK DV multiplications a head: 4 x 64
+// nodes of 48 heads 0.8 GFLOP).  Sums of g along a path are 64-bit, since differences of them are exponents.  Coefficients off a node's path
+// are exactly 0 and skipped, so that a node's values do not reach its siblings whatever they are.  A CTA runs through the code once, and
+// at small sizes fetching it is what takes the time: loops are kept rolled (66 KB of code unrolled: 18 us for four nodes).
 #include "sm100.cuh"
 
 namespace {
@@ -28,301 +34,452 @@ struct GdnTreeArgs {
   bf16* out; int64_t ldo;                 // [R * C, nv * dv]
   float* record;                          // [R, C, nv, dk + dv + 1]
   bf16* raw;                              // [R, C, conv]
-  int C, Cp, nk, nv, rep, nslots, gate_sigmoid;
+  float* rows;                            // [R, 2 nk + nv, C, d]: q heads, k heads, v heads
+  int R, C, Cp, nk, nv, rep, nslots, gate_sigmoid;
   float eps;
+};
+
+__device__ __forceinline__ uint64_t path_word(const GdnTreeArgs& a, int r, int j) {
+  const uint64_t on = (uint64_t)a.anc[(int64_t)r * a.C + j];
+  return on ? (on & (~0ull >> (63 - j))) | 1ull << j : 0;    // a path ends at its node
+}
+__device__ __forceinline__ bool unused(const GdnTreeArgs& a, int r) {
+  return a.slots[r] < 0 || a.slots[r] >= a.nslots || a.positions[r] < 0;
+}
+
+// ---- rows -----------------------------------------------------------------------------------
+template <int D>
+__global__ void __launch_bounds__(kThreads) gdn_tree_rows_kernel(const GdnTreeArgs a) {
+  constexpr int E = D / 32;
+  griddep_launch();
+  griddep_wait();
+  const int heads = 2 * a.nk + a.nv, lane = threadIdx.x & 31;
+  const int u = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), j = blockIdx.y, r = blockIdx.z;
+  if (u >= heads) return;
+  const uint64_t on = path_word(a, r, j);
+  if (on == 0 || unused(a, r)) return;
+  const int conv = heads * D, c = u * D + lane * E, pos = a.positions[r] + __popcll(on) - 1;
+  const bf16* ring = a.ring + (int64_t)a.slots[r] * kRing * conv + c;
+  const bf16* rows = a.proj + (int64_t)r * a.C * a.ldp + c;
+  uint32_t x[4][E / 2];
+  uint64_t up = on;
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {                              // the node, its parent, ...; behind the root the ring
+    const int node = up ? 63 - __clzll((long long)up) : -1;
+    if (up) up &= ~(1ull << node);
+    const bf16* from = node >= 0 ? rows + (int64_t)node * a.ldp : (pos >= b ? ring + (int64_t)((pos - b) & (kRing - 1)) * conv : nullptr);
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) x[b][e] = 0;
+    if (from) {
+      if (E == 4) *reinterpret_cast<uint2*>(x[b]) = *reinterpret_cast<const uint2*>(from);
+      else x[b][0] = *reinterpret_cast<const uint32_t*>(from);
+    }
+  }
+  bf16* raw = a.raw + ((int64_t)r * a.C + j) * conv + c;
+  if (E == 4) *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(x[0]);
+  else *reinterpret_cast<uint32_t*>(raw) = x[0][0];
+  float y[E], ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float4 w = *reinterpret_cast<const float4*>(a.conv_w + (int64_t)(c + e) * 4);
+    const auto f = [&](int b) { return __uint_as_float(e & 1 ? x[b][e / 2] & 0xffff0000u : x[b][e / 2] << 16); };
+    float v = w.x * f(3);
+    v = fmaf(w.y, f(2), v);
+    v = fmaf(w.z, f(1), v);
+    v = fmaf(w.w, f(0), v);
+    y[e] = v / (1.f + expf(-v));
+    ss = fmaf(y[e], y[e], ss);
+  }
+  if (u < 2 * a.nk) {
+    float f = rsqrtf(warp_sum(ss) + 1e-6f);
+    if (u < a.nk) f *= D == 128 ? 0.08838834764831845f : 0.125f;      // D^-0.5
+#pragma unroll
+    for (int e = 0; e < E; ++e) y[e] *= f;
+  }
+  float* to = a.rows + (((int64_t)r * heads + u) * a.C + j) * D + lane * E;
+  if (E == 4) *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(y);
+  else *reinterpret_cast<float2*>(to) = *reinterpret_cast<const float2*>(y);
+}
+
+// ---- nodes ----------------------------------------------------------------------------------
+// The products with the state: a warp keeps DK / SL channels of all DVS columns in registers, DVS / 32 columns a lane, and multiplies every
+// vector of its share with them (the vector's channels are the same for all lanes); the SL partial products meet in shared memory, BV
+// vectors at a time.  (What is left of it is bound by the loads of the vectors, 16 bytes a lane whether the lanes differ or not.)
+template <int DK, int DVS>
+struct TreeState {
+  static constexpr int WC = DVS / 32, SL = WC == 4 ? 8 : 4, VG = kThreads / 32 / SL, KR = DK / SL, BV = WC == 4 ? 8 : 32;
 };
 
 template <int DK, int DVS>
 struct TreeSmem {                         // floats
   static constexpr int LK = DK + 4;       // rows a quarter warp reads lie in different banks
-  int kn, qn, d, o, A, B, S, total;
+  int kn, qn, d, o, z, P, A, B, D, total; // z as bf16; A, B, D (and the doubling's scratch in D's place) follow the partial products in their place
   __host__ __device__ explicit TreeSmem(int Cp) {
     kn = 0;
     qn = kn + Cp * LK;
     d = qn + Cp * LK;
     o = d + Cp * DVS;
-    A = o + Cp * DVS;
+    z = o + Cp * DVS;
+    P = A = z + Cp * DVS / 2;
     B = A + Cp * (Cp + 4);
-    S = B + Cp * (Cp + 4);
-    total = S + DK * DVS;
+    D = B + Cp * (Cp + 4);
+    const int scratch = Cp * DVS > 32 * 36 ? Cp * DVS : 32 * 36;
+    const int bv = 2 * Cp < TreeState<DK, DVS>::BV ? 2 * Cp : TreeState<DK, DVS>::BV;
+    const int a = P + TreeState<DK, DVS>::SL * bv * DVS, b = D + scratch;
+    total = a > b ? a : b;
   }
 };
 
-// x_j += sum_i m[j][i] d_i over the nodes i < i1 for eight nodes j0 .. j0 + 7 of one column; places with m = 0 are off the path
-template <int DVS>
-__device__ __forceinline__ void add_nodes(float* x, const float* m, int ldm, const float* d, int j0, int i1, int col) {
+// x[j][.] += sum_{i < i1} m[j][i] y[i][.] for RT rows j and four columns; coefficients 0 are skipped
+template <int RT>
+__device__ __forceinline__ void rows_times(float (&x)[RT][4], const float* m, int ldm, const float* y, int ldy, int i1) {
+#pragma unroll 1
   for (int i = 0; i < i1; i += 4) {
-    float4 w[8];
-    bool any = false;
+    float4 w[RT], v[4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      w[j] = *reinterpret_cast<const float4*>(m + (j0 + j) * ldm + i);
-      any = any || w[j].x != 0.f || w[j].y != 0.f || w[j].z != 0.f || w[j].w != 0.f;
-    }
-    if (!any) continue;
-    float dv[4];
+    for (int j = 0; j < RT; ++j) w[j] = *reinterpret_cast<const float4*>(m + j * ldm + i);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) dv[e] = d[(i + e) * DVS + col];
+    for (int e = 0; e < 4; ++e) v[e] = *reinterpret_cast<const float4*>(y + (i + e) * ldy);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < RT; ++j) {
       const float f[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (f[e] != 0.f) x[j] = fmaf(f[e], dv[e], x[j]);
+        if (f[e] != 0.f) {
+          x[j][0] = fmaf(f[e], v[e].x, x[j][0]);
+          x[j][1] = fmaf(f[e], v[e].y, x[j][1]);
+          x[j][2] = fmaf(f[e], v[e].z, x[j][2]);
+          x[j][3] = fmaf(f[e], v[e].w, x[j][3]);
+        }
     }
   }
 }
 
-template <int DK, int DV, int DVS, int NVT>
+template <int NS>
+__device__ __forceinline__ void sync_all() {
+  if (NS > 1) sm100::cluster_sync_all();
+  else __syncthreads();
+}
+
+template <int DK, int DV, int DVS>
 __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a) {
-  constexpr int NS = DV / DVS, LK = TreeSmem<DK, DVS>::LK, NCH = (2 * DK + DVS) / 8;
+  constexpr int NS = DV / DVS, LK = TreeSmem<DK, DVS>::LK;
   extern __shared__ __align__(16) float sm[];
   __shared__ uint64_t anc_s[kMaxNodes];
-  __shared__ int up_s[kMaxNodes][3], depth_s[kMaxNodes];
   __shared__ double c_s[kMaxNodes];
-  __shared__ float g_s[kMaxNodes], beta_s[kMaxNodes], ss_s[kMaxNodes];
+  __shared__ __align__(16) float g_s[kMaxNodes];
+  __shared__ float beta_s[kMaxNodes], dec_s[kMaxNodes], ss_s[kMaxNodes];
   griddep_launch();
   griddep_wait();
   const int cg = blockIdx.x, h = blockIdx.y, r = blockIdx.z, kh = h / a.rep, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int slot = a.slots[r], pos0 = a.positions[r], C = a.C, Cp = a.Cp, LA = Cp + 4;
-  if (slot < 0 || slot >= a.nslots || pos0 < 0) return;      // the same for the whole cluster
+  const int C = a.C, Cp = a.Cp, LA = Cp + 4, heads = 2 * a.nk + a.nv;
   const TreeSmem<DK, DVS> off(Cp);
-  float *kn = sm + off.kn, *qn = sm + off.qn, *d = sm + off.d, *o = sm + off.o, *A = sm + off.A, *B = sm + off.B, *S = sm + off.S;
-  const int kdim = a.nk * DK, conv = 2 * kdim + a.nv * DV, col0 = cg * DVS;
-
-  // this CTA's columns of the state, on their way while the convolution runs
+  float *kn = sm + off.kn, *qn = sm + off.qn, *d = sm + off.d, *o = sm + off.o, *A = sm + off.A, *B = sm + off.B, *P = sm + off.P, *D = sm + off.D;
+  bf16* zs = reinterpret_cast<bf16*>(sm + off.z);
+  const int conv = 2 * a.nk * DK + a.nv * DV, col0 = cg * DVS;
+  auto copy16 = [](void* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sm100::smem_u32(to)), "l"(from));
+  };
+  // All that is read from memory is requested at once.  Rows without a node hold anything; they meet coefficients 0 alone.
+  const int slot = a.slots[r], pos0 = a.positions[r];
+  uint64_t on = 0;
+  float xb = 0.f, xa = 0.f;
+  if (tid < C) {
+    const bf16* row = a.proj + ((int64_t)r * C + tid) * a.ldp + conv + a.nv * DV;
+    on = path_word(a, r, tid);
+    xb = __bfloat162float(row[h]);
+    xa = __bfloat162float(row[a.nv + h]);
+  }
+  const float rate = a.A_log[h], dtb = a.dt_bias[h];
   {
-    const float* sp = a.state + ((int64_t)slot * a.nv + h) * DK * DV + col0;
-    for (int i = tid; i < DK * DVS / 4; i += kThreads) {
-      const int k = i / (DVS / 4), c = i % (DVS / 4) * 4;
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(sm100::smem_u32(S + k * DVS + c)), "l"(sp + (int64_t)k * DV + c));
+    const float* q = a.rows + ((int64_t)r * heads + kh) * C * DK;
+    const float* k = q + (int64_t)a.nk * C * DK;
+    const float* v = a.rows + ((int64_t)r * heads + 2 * a.nk + h) * C * DV + col0;
+#pragma unroll 1
+    for (int i = tid; i < C * DK / 4; i += kThreads) {
+      const int j = i / (DK / 4), c = i % (DK / 4) * 4;
+      copy16(kn + j * LK + c, k + j * DK + c);
+      copy16(qn + j * LK + c, q + j * DK + c);
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+#pragma unroll 1
+    for (int i = tid; i < C * DVS / 4; i += kThreads) {
+      const int j = i / (DVS / 4), c = i % (DVS / 4) * 4;
+      copy16(d + j * DVS + c, v + (int64_t)j * DV + c);
+    }
+    const bf16* z = a.proj + (int64_t)r * C * a.ldp + conv + h * DV + col0;
+#pragma unroll 1
+    for (int i = tid; i < C * DVS / 8; i += kThreads) {
+      const int j = i / (DVS / 8), c = i % (DVS / 8) * 8;
+      copy16(zs + j * DVS + c, z + j * a.ldp + c);
+    }
+  }
+  if (slot < 0 || slot >= a.nslots || pos0 < 0) {            // an unused row: the same for the whole cluster
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    return;
+  }
+  constexpr int WC = TreeState<DK, DVS>::WC, SL = TreeState<DK, DVS>::SL, VG = TreeState<DK, DVS>::VG, KR = TreeState<DK, DVS>::KR, BV = TreeState<DK, DVS>::BV;
+  const int sl = warp % SL;
+  float st[KR][WC];
+  {
+    const float* sp = a.state + (((int64_t)slot * a.nv + h) * DK + sl * KR) * DV + col0 + lane * WC;
+#pragma unroll
+    for (int k = 0; k < KR; ++k) {
+      if (WC == 4) *reinterpret_cast<float4*>(st[k]) = *reinterpret_cast<const float4*>(sp + k * DV);
+      else if (WC == 2) *reinterpret_cast<float2*>(st[k]) = *reinterpret_cast<const float2*>(sp + k * DV);
+      else st[k][0] = sp[k * DV];
+    }
   }
   if (tid < Cp) {
-    uint64_t on = 0;
-    if (tid < C) {
-      on = (uint64_t)a.anc[(int64_t)r * C + tid];
-      on = on ? (on & (~0ull >> (63 - tid))) | 1ull << tid : 0;
-    }
+    const float x = xa + dtb;
     anc_s[tid] = on;
-    depth_s[tid] = __popcll(on) - 1;
-    uint64_t up = on & ~(1ull << tid);
-#pragma unroll
-    for (int b = 0; b < 3; ++b) {
-      up_s[tid][b] = up ? 63 - __clzll((long long)up) : -1;
-      if (up) up &= ~(1ull << up_s[tid][b]);
-    }
-    float g = 0.f, beta = 0.f;
-    if (on) {
-      const bf16* row = a.proj + ((int64_t)r * C + tid) * a.ldp + conv + a.nv * DV;
-      const float x = __bfloat162float(row[a.nv + h]) + a.dt_bias[h];
-      g = fmaxf(-expf(a.A_log[h]) * (x > 20.f ? x : log1pf(expf(x))), -1e4f);      // exp of less is 0 all the same
-      beta = 1.f / (1.f + expf(-__bfloat162float(row[h])));
-    }
-    g_s[tid] = g;
-    beta_s[tid] = beta;
+    g_s[tid] = on ? fmaxf(-expf(rate) * (x > 20.f ? x : log1pf(expf(x))), -1e4f) : 0.f;      // exp of less is 0 all the same
+    beta_s[tid] = 1.f / (1.f + expf(-xb));
   }
   __syncthreads();
   if (tid < Cp) {
-    double c = 0.0;
-    for (uint64_t on = anc_s[tid]; on; on &= on - 1) c += (double)g_s[__ffsll((long long)on) - 1];
-    c_s[tid] = c;
-  }
-  // ---- convolution + SiLU: eight channels a thread, its weights in registers
-  if (tid < kThreads / NCH * NCH) {
-    const int ch = tid % NCH, x0 = ch * 8;
-    int c;                                                   // channel in the projection row
-    bool own;                                                // whose raw rows this CTA keeps
-    float* to;
-    int ldt;
-    if (x0 < DK) { c = kh * DK + x0; own = h % a.rep == 0 && cg == 0; to = qn + x0; ldt = LK; }
-    else if (x0 < 2 * DK) { c = kdim + kh * DK + x0 - DK; own = h % a.rep == 0 && cg == 0; to = kn + x0 - DK; ldt = LK; }
-    else { c = 2 * kdim + h * DV + col0 + x0 - 2 * DK; own = true; to = d + x0 - 2 * DK; ldt = DVS; }
-    float w[8][4];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) *reinterpret_cast<float4*>(w[i]) = *reinterpret_cast<const float4*>(a.conv_w + (int64_t)(c + i) * 4);
-    const bf16* ring = a.ring + (int64_t)slot * kRing * conv + c;
-    const bf16* rows = a.proj + (int64_t)r * C * a.ldp + c;
-    for (int j = tid / NCH; j < Cp; j += kThreads / NCH) {
-      float y[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = 0.f;
-      if (anc_s[j]) {
-#pragma unroll
-        for (int b = 3; b >= 0; --b) {                       // oldest tap first
-          const int node = b == 0 ? j : up_s[j][b - 1], pos = pos0 + depth_s[j] - b;
-          uint4 x = make_uint4(0, 0, 0, 0);
-          if (node >= 0) x = *reinterpret_cast<const uint4*>(rows + (int64_t)node * a.ldp);
-          else if (pos >= 0) x = *reinterpret_cast<const uint4*>(ring + (int64_t)(pos & (kRing - 1)) * conv);
-          if (b == 0 && own) *reinterpret_cast<uint4*>(a.raw + ((int64_t)r * C + j) * conv + c) = x;
-          float f[8];
-          bf16x8_to_float(x, f);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) y[i] = fmaf(w[i][3 - b], f[i], y[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = y[i] / (1.f + expf(-y[i]));
-      }
-      *reinterpret_cast<float4*>(to + j * ldt) = make_float4(y[0], y[1], y[2], y[3]);
-      *reinterpret_cast<float4*>(to + j * ldt + 4) = make_float4(y[4], y[5], y[6], y[7]);
+    double c[4] = {};
+#pragma unroll 1
+    for (int i = 0; on; i += 4, on >>= 4) {
+      const float4 g = *reinterpret_cast<const float4*>(g_s + i);
+      if (on & 1) c[0] += (double)g.x;
+      if (on & 2) c[1] += (double)g.y;
+      if (on & 4) c[2] += (double)g.z;
+      if (on & 8) c[3] += (double)g.w;
     }
-  }
-  __syncthreads();
-  // ---- norms of q and k
-  for (int j = warp; j < 2 * Cp; j += kThreads / 32) {
-    float* x = j < Cp ? kn + j * LK : qn + (j - Cp) * LK;
-    float ss = 0.f;
-    for (int i = lane; i < DK; i += 32) ss = fmaf(x[i], x[i], ss);
-    float f = 1.f / sqrtf(warp_sum(ss) + 1e-6f);
-    if (j >= Cp) f *= 1.f / sqrtf((float)DK);
-    for (int i = lane; i < DK; i += 32) x[i] *= f;
+    const double sum = (c[0] + c[1]) + (c[2] + c[3]);
+    c_s[tid] = sum;
+    dec_s[tid] = expf((float)sum);
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
-  // ---- S0^T k and S0^T q: four columns and NVT of the 2 Cp vectors a thread (row v < Cp of kn, then of qn)
-  {
-    constexpr int CG = DVS / 4, VL = kThreads / CG;
-    const int c4 = tid % CG * 4, v0 = tid / CG;
-    float acc[NVT][4];
-#pragma unroll
-    for (int n = 0; n < NVT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
+  // ---- S0^T k and S0^T q (vector v < Cp: row of kn, then of qn)
 #pragma unroll 1
-    for (int k = 0; k < DK; k += 4) {
-      float4 s[4];
+  for (int b0 = 0; b0 < 2 * Cp; b0 += BV) {
+    const int here = min(BV, 2 * Cp - b0);
+#pragma unroll 1
+    for (int v0 = (warp / SL) * 2; v0 < here; v0 += 2 * VG) {        // two vectors at a time (their number is even)
+      const int v = b0 + v0;
+      const float* x = (v < Cp ? kn + v * LK : qn + (v - Cp) * LK) + sl * KR;
+      float acc[2][WC];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[e] = *reinterpret_cast<const float4*>(S + (k + e) * DVS + c4);
+      for (int c = 0; c < WC; ++c) acc[0][c] = acc[1][c] = 0.f;
 #pragma unroll
-      for (int n = 0; n < NVT; ++n) {
-        const int v = v0 + n * VL;
-        if (v < 2 * Cp) {
-          const float4 x = *reinterpret_cast<const float4*>((v < Cp ? kn + v * LK : qn + (v - Cp) * LK) + k);
-          const float f[4] = {x.x, x.y, x.z, x.w};
+      for (int k = 0; k < KR; k += 4) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            acc[n][0] = fmaf(f[e], s[e].x, acc[n][0]);
-            acc[n][1] = fmaf(f[e], s[e].y, acc[n][1]);
-            acc[n][2] = fmaf(f[e], s[e].z, acc[n][2]);
-            acc[n][3] = fmaf(f[e], s[e].w, acc[n][3]);
+        for (int n = 0; n < 2; ++n) {
+          const float4 f = *reinterpret_cast<const float4*>(x + n * LK + k);
+#pragma unroll
+          for (int c = 0; c < WC; ++c) {
+            acc[n][c] = fmaf(f.x, st[k][c], acc[n][c]);
+            acc[n][c] = fmaf(f.y, st[k + 1][c], acc[n][c]);
+            acc[n][c] = fmaf(f.z, st[k + 2][c], acc[n][c]);
+            acc[n][c] = fmaf(f.w, st[k + 3][c], acc[n][c]);
           }
         }
       }
-    }
 #pragma unroll
-    for (int n = 0; n < NVT; ++n) {
-      const int v = v0 + n * VL, j = v < Cp ? v : v - Cp;
-      if (v >= 2 * Cp) continue;
-      const float f = (float)exp(c_s[j]), b = beta_s[j];
-      float* x = (v < Cp ? d : o) + j * DVS + c4;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[e] = v < Cp ? b * (x[e] - f * acc[n][e]) : f * acc[n][e];
+      for (int n = 0; n < 2; ++n) {
+        float* to = P + (sl * here + v0 + n) * DVS + lane * WC;
+        if (WC == 4) *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(acc[n]);
+        else if (WC == 2) *reinterpret_cast<float2*>(to) = *reinterpret_cast<const float2*>(acc[n]);
+        else to[0] = acc[n][0];
+      }
     }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < here * DVS / 4; i += kThreads) {
+      float4 s = *reinterpret_cast<const float4*>(P + i * 4);
+#pragma unroll
+      for (int n = 1; n < SL; ++n) {
+        const float4 p = *reinterpret_cast<const float4*>(P + n * here * DVS + i * 4);
+        s.x += p.x; s.y += p.y; s.z += p.z; s.w += p.w;
+      }
+      const int v = b0 + i / (DVS / 4), j = v < Cp ? v : v - Cp, c = i % (DVS / 4) * 4;
+      const float f = dec_s[j], b = beta_s[j];
+      float4* x = reinterpret_cast<float4*>((v < Cp ? d : o) + j * DVS + c);
+      if (v < Cp) {
+        const float4 w = *x;
+        *x = make_float4(b * (w.x - f * s.x), b * (w.y - f * s.y), b * (w.z - f * s.z), b * (w.w - f * s.w));
+      } else *x = make_float4(f * s.x, f * s.y, f * s.z, f * s.w);
+    }
+    if (b0 + BV < 2 * Cp) __syncthreads();
   }
-  // ---- Gram matrices: A_ji = -beta_j e^{c_j - c_i} k_j.k_i above j, B_ji = e^{c_j - c_i} q_j.k_i above j and at j; 0 elsewhere
-  for (int t = tid; t < Cp * Cp / 4; t += kThreads) {        // two rows j, two columns i a thread
-    const int half = Cp / 2, i0 = t % half, j0 = t / half;
-    float kk[2][2] = {}, qk[2][2] = {};
-    const bool low = j0 + half >= i0;
-    if (low) {
-      for (int k = 0; k < DK; k += 4) {
-        float4 x[2], y[2], z[2];
+  sync_all<NS>();                                            // the partial products' place is free, in every CTA of the cluster
+  // ---- Gram matrices: A_ji = -beta_j e^{c_j - c_i} k_j.k_i above j, B_ji = e^{c_j - c_i} q_j.k_i above j and at j; 0 elsewhere.  Units of
+  // 4 x 4 on and below the diagonal, four threads (a quarter of the channels each) a unit; the CTAs of a cluster take every NS-th unit.
+  {
+    const int nb = Cp / 4, units = nb * (nb + 1) / 2, part = tid & 3;
+    const unsigned four = 0xfu << (lane & 28);
+#pragma unroll 1
+    for (int u = tid; u < Cp * nb; u += kThreads)            // above the diagonal blocks A is 0; B is not read there
+      if (u % nb > u / nb / 4) *reinterpret_cast<float4*>(A + u / nb * LA + u % nb * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+    for (int u = (tid >> 2) * NS + cg; u < units; u += kThreads / 4 * NS) {        // the four threads of a unit stay together
+      const int jb = (int)((sqrtf((float)(8 * u + 1)) - 1.f) * 0.5f), j0 = jb * 4, i0 = (u - jb * (jb + 1) / 2) * 4;      // exact: u <= 135
+      float g[2][4][4];                                      // k_j.k_i, q_j.k_i
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          x[e] = *reinterpret_cast<const float4*>(kn + (i0 + e * half) * LK + k);
-          y[e] = *reinterpret_cast<const float4*>(kn + (j0 + e * half) * LK + k);
-          z[e] = *reinterpret_cast<const float4*>(qn + (j0 + e * half) * LK + k);
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) g[0][x][y] = g[1][x][y] = 0.f;
+#pragma unroll 1
+      for (int k = part * 4; k < DK; k += 16) {              // quarters interleaved by 16 bytes: the four threads read neighbours
+        float4 ki[4];
+#pragma unroll
+        for (int y = 0; y < 4; ++y) ki[y] = *reinterpret_cast<const float4*>(kn + (i0 + y) * LK + k);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float4 kj = *reinterpret_cast<const float4*>(kn + (j0 + x) * LK + k), qj = *reinterpret_cast<const float4*>(qn + (j0 + x) * LK + k);
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            g[0][x][y] = fmaf(kj.x, ki[y].x, fmaf(kj.y, ki[y].y, fmaf(kj.z, ki[y].z, fmaf(kj.w, ki[y].w, g[0][x][y]))));
+            g[1][x][y] = fmaf(qj.x, ki[y].x, fmaf(qj.y, ki[y].y, fmaf(qj.z, ki[y].z, fmaf(qj.w, ki[y].w, g[1][x][y]))));
+          }
+        }
+      }
+      // the four quarters are added so that thread x of the four ends up with row x: first pairs of rows, then rows
+      const int j = j0 + part;
+      const bool hi = part & 2, odd = part & 1;
+      float row[2][4];
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+          const float s0 = __shfl_xor_sync(four, hi ? g[w][0][y] : g[w][2][y], 2), s1 = __shfl_xor_sync(four, hi ? g[w][1][y] : g[w][3][y], 2);
+          const float a0 = (hi ? g[w][2][y] : g[w][0][y]) + s0, a1 = (hi ? g[w][3][y] : g[w][1][y]) + s1;
+          row[w][y] = (odd ? a1 : a0) + __shfl_xor_sync(four, odd ? a0 : a1, 1);
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int v = 0; v < 2; ++v) {
-            kk[u][v] += y[u].x * x[v].x + y[u].y * x[v].y + y[u].z * x[v].z + y[u].w * x[v].w;
-            qk[u][v] += z[u].x * x[v].x + z[u].y * x[v].y + z[u].z * x[v].z + z[u].w * x[v].w;
-          }
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int v = 0; v < 2; ++v) {
-        const int j = j0 + u * half, i = i0 + v * half;
+      for (int y = 0; y < 4; ++y) {
+        const int i = i0 + y;
         const bool on = anc_s[j] >> i & 1;
-        const float f = on ? (float)exp(c_s[j] - c_s[i]) : 0.f;
-        A[j * LA + i] = on && i != j ? -beta_s[j] * f * kk[u][v] : 0.f;
-        B[j * LA + i] = on ? f * qk[u][v] : 0.f;
+        const float f = on ? expf((float)(c_s[j] - c_s[i])) : 0.f;
+        row[0][y] = on && i != j ? -beta_s[j] * f * row[0][y] : 0.f;
+        row[1][y] = on ? f * row[1][y] : 0.f;
       }
-  }
-  __syncthreads();
-  // ---- d: blocks of eight nodes; what comes from earlier blocks first, then eight steps within the block.  o follows with the d's of
-  // its own block.
-  for (int j0 = 0; j0 < Cp; j0 += 8) {
-    if (tid < DVS) {
-      float x[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = d[(j0 + j) * DVS + tid];
-      add_nodes<DVS>(x, A, LA, d, j0, j0, tid);
+      for (int w = 0; w < 2; ++w) {
+        float* to = (w ? B : A) + j * LA + i0;
+        if (NS == 1) *reinterpret_cast<float4*>(to) = make_float4(row[w][0], row[w][1], row[w][2], row[w][3]);
+        else {
 #pragma unroll
-      for (int j = 1; j < 8; ++j)
-#pragma unroll
-        for (int i = 0; i < j; ++i) {
-          const float f = A[(j0 + j) * LA + j0 + i];
-          if (f != 0.f) x[j] = fmaf(f, x[i], x[j]);
+          for (int n = 0; n < NS; ++n)
+            asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(sm100::map_to_cta(sm100::smem_u32(to), n)), "f"(row[w][0]), "f"(row[w][1]),
+                         "f"(row[w][2]), "f"(row[w][3]) : "memory");
         }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) d[(j0 + j) * DVS + tid] = x[j];
+      }
     }
   }
-  __syncthreads();
-  for (int t = tid; t < Cp / 8 * DVS; t += kThreads) {
-    const int col = t % DVS, j0 = t / DVS * 8;
-    float x[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) x[j] = o[(j0 + j) * DVS + col];
-    add_nodes<DVS>(x, B, LA, d, j0, j0 + 8, col);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[(j0 + j) * DVS + col] = x[j];
+  sync_all<NS>();
+  // ---- M = (1 - A)^-1 in A's place: 4 x 4 blocks on the diagonal, a thread a column, then M21 = M22 A21 M11 by doubling
+  if (tid < Cp) {
+    const int i = tid % 4;
+    float* x = A + (tid / 4 * 4) * LA + tid / 4 * 4;         // strictly lower: x10, x20, x21, x30, x31, x32
+    const float x10 = x[LA], x20 = x[2 * LA], x21 = x[2 * LA + 1], x30 = x[3 * LA], x31 = x[3 * LA + 1], x32 = x[3 * LA + 2];
+    __syncwarp(Cp - warp * 32 >= 32 ? 0xffffffffu : (1u << (Cp - warp * 32)) - 1);      // all four have read before one writes
+    auto times = [](float f, float y) { return f != 0.f && y != 0.f ? f * y : 0.f; };
+    const float m0 = i == 0 ? 1.f : 0.f;
+    const float m1 = i == 1 ? 1.f : times(x10, m0);
+    const float m2 = i == 2 ? 1.f : times(x20, m0) + times(x21, m1);
+    const float m3 = i == 3 ? 1.f : times(x30, m0) + times(x31, m1) + times(x32, m2);
+    x[i] = m0;
+    x[LA + i] = m1;
+    x[2 * LA + i] = m2;
+    x[3 * LA + i] = m3;
   }
   __syncthreads();
+#pragma unroll 1
+  for (int n = 4; n < Cp; n *= 2) {                          // pairs of n x n blocks: rows [p + n, p + 2 n), columns [p, p + n)
+    const int q = n / 4, units = n * q;                      // a row and four columns a thread
+    const int u = tid % units, p = tid / units * 2 * n, x0 = u / q, y0 = u % q * 4;
+    const bool mine = p + n < Cp && x0 < Cp - p - n;
+    float* low = A + (p + n + x0) * LA + p;                  // this row of the lower block, first column of the pair
+    float* t = D + tid / units * n * (n + 4);                // [n][n + 4] a pair: A21 M11
+#pragma unroll 1
+    for (int s = 0; s < 2; ++s) {
+      float x[1][4] = {};
+      if (mine) rows_times(x, s ? low + n : low, 0, s ? t + y0 : A + p * LA + p + y0, s ? n + 4 : LA, s ? x0 / 4 * 4 + 4 : n);
+      __syncthreads();                                       // A21 has been read before it is written
+      if (mine) *reinterpret_cast<float4*>(s ? low + y0 : t + x0 * (n + 4) + y0) = make_float4(x[0][0], x[0][1], x[0][2], x[0][3]);
+      __syncthreads();
+    }
+  }
+  // ---- updates D = M W and outputs O += B D with their squares, four rows and four columns a thread
+#pragma unroll 1
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll 1
+    for (int u = tid; u < Cp / 4 * (DVS / 4); u += kThreads) {
+      const int c4 = u % (DVS / 4) * 4, j0 = u / (DVS / 4) * 4;
+      float x[4][4] = {};
+      if (pass) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *reinterpret_cast<float4*>(x[e]) = *reinterpret_cast<const float4*>(o + (j0 + e) * DVS + c4);
+      }
+      rows_times(x, (pass ? B : A) + j0 * LA, LA, (pass ? D : d) + c4, DVS, j0 + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) *reinterpret_cast<float4*>((pass ? o : D) + (j0 + e) * DVS + c4) = make_float4(x[e][0], x[e][1], x[e][2], x[e][3]);
+      if (pass) {                                            // DVS / 4 neighbouring lanes hold a row's columns, all of them or none
+        const unsigned lanes = DVS == 128 ? 0xffffffffu : ((1u << (DVS / 4)) - 1) << (lane / (DVS / 4) * (DVS / 4));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float ss = fmaf(x[e][0], x[e][0], fmaf(x[e][1], x[e][1], fmaf(x[e][2], x[e][2], x[e][3] * x[e][3])));
+#pragma unroll
+          for (int w = DVS / 8; w > 0; w >>= 1) ss += __shfl_xor_sync(lanes, ss, w);
+          if (c4 == 0) ss_s[j0 + e] = ss;
+        }
+      }
+    }
+    __syncthreads();
+  }
   // ---- norm over the head's columns, gate, record
-  for (int j = warp; j < C; j += kThreads / 32) {
-    float ss = 0.f;
-    for (int i = lane; i < DVS; i += 32) ss = fmaf(o[j * DVS + i], o[j * DVS + i], ss);
-    ss = warp_sum(ss);
-    if (lane == 0) ss_s[j] = ss;
-  }
-  if (NS > 1) sm100::cluster_sync_all();
-  else __syncthreads();
-  for (int j = warp; j < C; j += kThreads / 32) {
-    if (!anc_s[j]) continue;
-    float ss = 0.f;
+  sync_all<NS>();
+  if (tid < C) {
+    float ss = ss_s[tid];
     if (NS > 1) {
+      ss = 0.f;
 #pragma unroll
       for (int n = 0; n < NS; ++n) {                         // the same order in every CTA
         float v;
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(sm100::map_to_cta(sm100::smem_u32(ss_s + j), n)) : "memory");
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(sm100::map_to_cta(sm100::smem_u32(ss_s + tid), n)) : "memory");
         ss += v;
       }
-    } else ss = ss_s[j];
-    const float f = 1.f / sqrtf(ss / (float)DV + a.eps);
-    const int64_t row = (int64_t)r * C + j;
-    const bf16* z = a.proj + row * a.ldp + conv + h * DV + col0;
-    float* rec = a.record + (row * a.nv + h) * (DK + DV + 1);
-    for (int i = lane; i < DVS; i += 32) {
-      const float x = __bfloat162float(z[i]), s = 1.f / (1.f + expf(-x));
-      a.out[row * a.ldo + h * DV + col0 + i] = __float2bfloat16(o[j * DVS + i] * f * a.norm_w[col0 + i] * (a.gate_sigmoid ? s : x * s));
-      rec[DK + col0 + i] = d[j * DVS + i];
     }
-    if (cg == 0) {
-      for (int i = lane; i < DK; i += 32) rec[i] = kn[j * LK + i];
-      if (lane == 0) rec[DK + DV] = expf(g_s[j]);
-    }
+    dec_s[tid] = rsqrtf(ss * (1.f / DV) + a.eps);
+    if (cg == 0 && anc_s[tid]) a.record[(((int64_t)r * C + tid) * a.nv + h) * (DK + DV + 1) + DK + DV] = expf(g_s[tid]);
   }
   if (NS > 1) sm100::cluster_sync_all();                     // nobody leaves while its sums may still be read
+  else __syncthreads();
+  const float4 nw = *reinterpret_cast<const float4*>(a.norm_w + col0 + tid % (DVS / 4) * 4);
+#pragma unroll 1
+  for (int i = tid; i < C * (DVS / 4); i += kThreads) {
+    const int j = i / (DVS / 4), c = i % (DVS / 4) * 4;      // the same columns in every turn
+    if (!anc_s[j]) continue;
+    const int64_t row = (int64_t)r * C + j;
+    const float4 x = *reinterpret_cast<const float4*>(o + j * DVS + c), u = *reinterpret_cast<const float4*>(D + j * DVS + c);
+    const uint2 zb = *reinterpret_cast<const uint2*>(zs + j * DVS + c);
+    const float z[4] = {__uint_as_float(zb.x << 16), __uint_as_float(zb.x & 0xffff0000u), __uint_as_float(zb.y << 16), __uint_as_float(zb.y & 0xffff0000u)};
+    float y[4] = {x.x * nw.x, x.y * nw.y, x.z * nw.z, x.w * nw.w};
+    const float f = dec_s[j];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float s = 1.f / (1.f + expf(-z[e]));
+      y[e] *= f * (a.gate_sigmoid ? s : z[e] * s);
+    }
+    bf16* out = a.out + row * a.ldo + h * DV + col0 + c;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf162(y[0], y[1]), pack_bf162(y[2], y[3]));
+    float* rec = a.record + (row * a.nv + h) * (DK + DV + 1) + DK + col0 + c;
+    rec[0] = u.x; rec[1] = u.y; rec[2] = u.z; rec[3] = u.w;
+  }
+  constexpr int KS = DK / NS;                                // the CTAs of a cluster share the copy of the keys
+#pragma unroll 4
+  for (int i = tid; i < C * KS; i += kThreads) {
+    const int j = i / KS, c = cg * KS + i % KS;
+    if (anc_s[j]) a.record[(((int64_t)r * C + j) * a.nv + h) * (DK + DV + 1) + c] = kn[j * LK + c];
+  }
 }
 
-template <int DK, int DV, int DVS, int NVT>
+template <int DK, int DV, int DVS>
 int launch_gdn_tree(const GdnTreeArgs& a, int R, cudaStream_t st) {
-  auto kern = gdn_tree_kernel<DK, DV, DVS, NVT>;
+  auto kern = gdn_tree_kernel<DK, DV, DVS>;
   const size_t smem = TreeSmem<DK, DVS>(a.Cp).total * sizeof(float);
   cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
   if (e != cudaSuccess) return (int)e;
@@ -342,31 +499,28 @@ int launch_gdn_tree(const GdnTreeArgs& a, int R, cudaStream_t st) {
   return (int)cudaLaunchKernelEx(&cfg, kern, a);
 }
 
-template <int DK, int DV, int DVS>
-int pick_nodes(const GdnTreeArgs& a, int R, cudaStream_t st) {
-  constexpr int VL = kThreads / (DVS / 4);                   // vectors side by side
-  const int need = (2 * a.Cp + VL - 1) / VL;
-  if (need <= 1) return launch_gdn_tree<DK, DV, DVS, 1>(a, R, st);
-  if (need <= 2) return launch_gdn_tree<DK, DV, DVS, 2>(a, R, st);
-  if (need <= 4) return launch_gdn_tree<DK, DV, DVS, 4>(a, R, st);
-  if (need <= 8) return launch_gdn_tree<DK, DV, DVS, 8>(a, R, st);
-  return need <= 16 ? launch_gdn_tree<DK, DV, DVS, 16>(a, R, st) : CB_ERR_SHAPE;
-}
-
 }  // namespace
 
 CB_EXPORT int cb_gdn_tree(const void* proj, int64_t ldp, const void* conv_w, const void* A_log, const void* dt_bias, const void* norm_w,
                           const void* ring, const void* state, const void* slots, const void* positions, const void* anc, void* out, int64_t ldo,
-                          void* record, void* raw, int64_t nslots, int64_t R, int64_t C, int64_t nk, int64_t nv, int64_t dk, int64_t dv, float eps,
+                          void* record, void* raw, void* rows, int64_t nslots, int64_t R, int64_t C, int64_t nk, int64_t nv, int64_t dk, int64_t dv, float eps,
                           int64_t gate_sigmoid, void* stream) {
-  if (!proj || !conv_w || !A_log || !dt_bias || !norm_w || !ring || !state || !slots || !positions || !anc || !out || !record || !raw) return CB_ERR_ARG;
-  if (R < 1 || R > 65535 || C < 1 || C > kMaxNodes || nk < 1 || nv % nk || nv > 65535 || ldp % 8 ||
-      (((uintptr_t)proj | (uintptr_t)ring | (uintptr_t)state | (uintptr_t)raw | (uintptr_t)conv_w) & 15)) return CB_ERR_SHAPE;
+  if (!proj || !conv_w || !A_log || !dt_bias || !norm_w || !ring || !state || !slots || !positions || !anc || !out || !record || !raw || !rows) return CB_ERR_ARG;
+  if (R < 1 || R > 65535 || C < 1 || C > kMaxNodes || nk < 1 || nv % nk || nv > 65535 || ldp % 8 || ldo % 4 || ((uintptr_t)out & 7) || ((uintptr_t)norm_w & 15) ||
+      (((uintptr_t)proj | (uintptr_t)ring | (uintptr_t)state | (uintptr_t)raw | (uintptr_t)rows | (uintptr_t)conv_w) & 15)) return CB_ERR_SHAPE;
   GdnTreeArgs a{(const bf16*)proj, ldp, (const float*)conv_w, (const float*)A_log, (const float*)dt_bias, (const float*)norm_w, (const bf16*)ring,
-                (const float*)state, (const int*)slots, (const int*)positions, (const int64_t*)anc, (bf16*)out, ldo, (float*)record, (bf16*)raw,
-                (int)C, (int)((C + 7) / 8 * 8), (int)nk, (int)nv, (int)(nv / nk), (int)nslots, (int)gate_sigmoid, eps};
+                (const float*)state, (const int*)slots, (const int*)positions, (const int64_t*)anc, (bf16*)out, ldo, (float*)record, (bf16*)raw, (float*)rows,
+                (int)R, (int)C, (int)((C + 7) / 8 * 8), (int)nk, (int)nv, (int)(nv / nk), (int)nslots, (int)gate_sigmoid, eps};
   cudaStream_t st = (cudaStream_t)stream;
-  if (dk == 128 && dv == 128) return pick_nodes<128, 128, 64>(a, (int)R, st);
-  if (dk == 64 && dv == 64) return pick_nodes<64, 64, 32>(a, (int)R, st);
-  return CB_ERR_SHAPE;
+  if (!((dk == 128 && dv == 128) || (dk == 64 && dv == 64))) return CB_ERR_SHAPE;
+  const dim3 grid((unsigned)((2 * nk + nv + kThreads / 32 - 1) / (kThreads / 32)), (unsigned)C, (unsigned)R);
+  cudaError_t e = dk == 128 ? cb_launch(gdn_tree_rows_kernel<128>, grid, dim3(kThreads), 0, st, a) : cb_launch(gdn_tree_rows_kernel<64>, grid, dim3(kThreads), 0, st, a);
+  if (e != cudaSuccess) return (int)e;
+  // A head's columns are split over a cluster while all CTAs still run at once.  us of 1 / 2 / 4 CTAs a head: 16 nodes, 32 heads 21.1 / 18.0 /
+  // 17.9, 128 heads 23.9 / 20.9 / 32.6, 256 heads 25.6 / 35.4 / 47.2; 64 nodes, 32 heads 49.9 / 36.0 / 30.3, 192 heads 106.7 / 106.4 / 156.4.
+  // Up to eight nodes the exchange costs more than it saves: 4 nodes, 32 heads 11.8 / 12.8 / 13.3.
+  const int64_t room = 148 / (R * nv);
+  const int ns = C <= 8 || room < 2 ? 1 : (room < 4 ? 2 : 4);
+  if (dk == 128) return ns == 1 ? launch_gdn_tree<128, 128, 128>(a, (int)R, st) : ns == 2 ? launch_gdn_tree<128, 128, 64>(a, (int)R, st) : launch_gdn_tree<128, 128, 32>(a, (int)R, st);
+  return launch_gdn_tree<64, 64, 32>(a, (int)R, st);              // two CTAs a head
 }

@@ -106,21 +106,24 @@ def gdn_tree(proj, conv_w, A_log, dt_bias, norm_w, ring, state, slots, positions
     _need((dk, dv) in ((128, 128), (64, 64)) and nk >= 1 and nv % nk == 0, f"delta-net heads {nk} / {nv} of {dk} x {dv}")
     _need(proj.dtype == bf and proj.dim() == 2 and proj.shape[0] >= R * C and proj.shape[1] >= conv + nv * dv + 2 * nv and proj.stride(1) == 1
           and proj.stride(0) % 8 == 0 and proj.data_ptr() % 16 == 0, "proj: bf16 rows q | k | v | z | b | a of a multiple of 16 bytes")
-    _need(out.dtype == bf and out.dim() == 2 and out.shape[0] >= R * C and out.shape[1] >= nv * dv and out.stride(1) == 1, "out: bf16 [R * C, nv * dv]")
+    _need(out.dtype == bf and out.dim() == 2 and out.shape[0] >= R * C and out.shape[1] >= nv * dv and out.stride(1) == 1
+          and out.stride(0) % 4 == 0 and out.data_ptr() % 8 == 0, "out: bf16 [R * C, nv * dv] in 8-byte rows")
     n = state.shape[0]
     _need(state.dtype == f32 and state.shape == (n, nv, dk, dv) and state.is_contiguous() and state.data_ptr() % 16 == 0, "state: contiguous fp32 [slots, nv, dk, dv]")
     _need(ring.dtype == bf and ring.shape == (n, K.RING, conv) and ring.is_contiguous() and ring.data_ptr() % 16 == 0, "ring: contiguous bf16 [slots, 16, conv]")
     _vec(conv_w, conv * 4, f32, "conv_w")
     _need(conv_w.data_ptr() % 16 == 0, "conv_w: 16-byte rows")
     _vec(A_log, nv, f32, "A_log"), _vec(dt_bias, nv, f32, "dt_bias"), _vec(norm_w, dv, f32, "norm_w")
+    _need(norm_w.data_ptr() % 16 == 0, "norm_w: a 16-byte address")
     _vec(slots, R, torch.int32, "slots"), _vec(positions, R, torch.int32, "positions")
     _vec(record, R * C * nv * (dk + dv + 1), f32, "record"), _vec(raw, R * C * conv, bf, "raw")
     _place(proj, conv_w=conv_w, A_log=A_log, dt_bias=dt_bias, norm_w=norm_w, ring=ring, state=state, slots=slots, positions=positions, anc=anc,
            out=out, record=record, raw=raw)
     if R:
-        call("gdn_tree", proj, proj.stride(0), conv_w, A_log, dt_bias, norm_w, ring, state, slots, positions, anc, out, out.stride(0), record, raw,
+        rows = torch.empty(R * C * conv, dtype=f32, device=proj.device)
+        call("gdn_tree", proj, proj.stride(0), conv_w, A_log, dt_bias, norm_w, ring, state, slots, positions, anc, out, out.stride(0), record, raw, rows,
              n, R, C, nk, nv, dk, dv, float(eps), int(gate_sigmoid))
-        K._count()
+        K._count(2)
     return out
 
 
