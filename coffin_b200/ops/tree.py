@@ -228,7 +228,7 @@ def gdn_tree_commit(state, ring, record, raw, slots, positions, path, steps, *, 
     them.  Sequence ``r`` is read in slot ``slots[r]`` (< 0: unused row) and written in ``to_slots[r]`` (the same ones by default; all
     slots that are written are distinct and none of them is read for another sequence)."""
     R, C = _path(path, steps, positions)
-    _need(state.dim() == 5 and state.dtype == torch.float32 and state.is_contiguous(), "state: contiguous fp32 [layers, slots, nv, dk, dv]")
+    _need(state.dim() == 5 and state.dtype == torch.float32 and state.is_contiguous() and state.data_ptr() % 16 == 0, "state: contiguous fp32 [layers, slots, nv, dk, dv]")
     L, n, nv, dk, dv = state.shape
     _need((dk, dv) in ((128, 128), (64, 64)), f"delta-net states of {dk} x {dv}")
     conv = ring.shape[-1]

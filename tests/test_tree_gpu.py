@@ -375,6 +375,24 @@ def test_verification_with_masked_vocabularies_and_uniforms_at_the_ends():
     assert 0 <= t < V
 
 
+@pytest.mark.parametrize("T", [1e-30, 1e-9, 3e-5, 0.02, 50.0, 1e30])
+def test_verification_at_every_temperature(T):
+    """Very cold rows are the arg-max (or one of its equals), very hot ones uniform over what is not masked."""
+    from coffin_b200.ops import tree
+    R, V = 6, 5001
+    logits = torch.randn(R, 1, V, generator=_gen(11), device="cuda") * 4 + 31.0
+    logits[1] -= 62.0
+    logits[2, 0, [7, 4500]] = logits[2].max() + 1
+    logits[3, 0, ::3] = float("-inf")
+    temps = torch.full((R,), T, device="cuda")
+    u = torch.rand(R, 1, generator=_gen(12), device="cuda")
+    one = torch.ones(R, 1, dtype=I64, device="cuda")
+    got = tree.verify_tree(logits, one, one, temps, u)[2].tolist()
+    for r in range(R):
+        want, near = P.choose(P.probs(logits[r, 0], float(temps[r])), float(u[r, 0]))
+        assert near > 1e-11 and got[r] == want, r
+
+
 def test_verification_skips_unused_sequences_and_reads_strided_logits():
     from coffin_b200.ops import tree
     logits, parents, tokens, temps, u = _trees(3, 6, 1003, 0.8, 5)
