@@ -262,6 +262,8 @@ class LLMEngine:
         should run instead (no drafts, no room for the draft window)."""
         if not (self.cfg.spec_k > 0 or any(s.params.spec_k > 0 for s in ready)):
             return False
+        if self.runner.tree_drafts:
+            return self._run_tree(ready, tokens, out)
         drafts = self.runner.draft(ready)
         if drafts is None:
             return False
@@ -277,6 +279,22 @@ class LLMEngine:
             for i, tok in zip(idx, picked):
                 new_tokens[i] = [tok]
         for seq, toks in zip(ready, new_tokens):
+            for tok in toks:
+                self._commit(seq, tok, out)
+                if seq.finished:
+                    break
+        return True
+
+    def _run_tree(self, ready: list[Sequence], tokens: list[int], out: list[StepOutput]) -> bool:
+        """Speculative step over trees of drafts: every row's own tokens (arg-max, or drawn with its uniforms) are followed through its
+        tree, so sampled rows take part like greedy ones."""
+        trees = self.runner.draft_trees(ready)
+        if trees is None:
+            return False
+        for seq, (drafts, _p) in zip(ready, trees):
+            if seq.num_computed + len(drafts) + 1 > self.max_seq or not self.bm.ensure_blocks(seq.blocks, len(drafts) + 1):
+                return False
+        for seq, toks in zip(ready, self.runner.tree_step(ready, tokens, trees)):
             for tok in toks:
                 self._commit(seq, tok, out)
                 if seq.finished:

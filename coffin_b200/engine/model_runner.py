@@ -315,8 +315,8 @@ class ModelRunner:
 
     def spec_k_of(self, seq: Sequence) -> int:
         """Draft length of a row: the request's own ``spec_k`` or the engine default; rows that sample
-        with a temperature cannot be verified by arg-max and never draft."""
-        if seq.params.temperature > 0 or not self.spec_capable:
+        with a temperature cannot be verified by arg-max and draft only where their draws are compared (``spec_sample``)."""
+        if not self.spec_capable or (seq.params.temperature > 0 and not (self.cfg.spec_sample and self.tree_capable)):
             return 0
         k = seq.params.spec_k if seq.params.spec_k >= 0 else self.cfg.spec_k
         if seq.num_tokens < self.cfg.spec_min_ctx:
@@ -346,6 +346,78 @@ class ModelRunner:
             drafts.append(d)
             any_draft = any_draft or bool(d)
         return drafts if any_draft else None
+
+    # ------------------------------------------------------------------ trees of drafts
+    @property
+    def tree_capable(self) -> bool:
+        return hasattr(self.model, "verify_tree")
+
+    @property
+    def tree_drafts(self) -> bool:
+        """Whether speculative steps verify trees (a chain is one): branching drafts, or rows that are sampled."""
+        return self.tree_capable and (self.cfg.spec_tree > 0 or self.cfg.spec_sample)
+
+    TREE_ROWS = 64            # token rows of one verify pass
+
+    def draft_trees(self, seqs: list[Sequence]) -> list[tuple[list[int], list[int]]] | None:
+        """Drafted ``(tokens, parents)`` of every row (parent -1: behind the row's pending token); ``None`` when no row drafts."""
+        from ..utils.suffix import SuffixDrafter
+        if len(seqs) > self.SPEC_MAX_ROWS or not (self.cfg.spec_batch or len(seqs) == 1):
+            return None
+        rows = 1
+        while rows < len(seqs):
+            rows *= 2
+        trees = []
+        for s in seqs:
+            k = self.spec_k_of(s)
+            room = min(self.TREE_ROWS // rows - 1, (self.model.max_seq if hasattr(self.model, "max_seq") else 1 << 30) - s.num_tokens - 1)
+            if k <= 0 or room <= 0:
+                trees.append(([], []))
+                continue
+            if s.drafter is None:
+                s.drafter, s.drafter_seen = SuffixDrafter(), 0
+            toks = s.all_tokens
+            if s.drafter_seen < len(toks):
+                s.drafter.observe(toks[s.drafter_seen:])
+                s.drafter_seen = len(toks)
+            trees.append(s.drafter.draft_tree(k, min(room, self.cfg.spec_tree if self.cfg.spec_tree > 0 else k)))
+        return trees if any(t for t, _p in trees) else None
+
+    def tree_step(self, seqs: list[Sequence], tokens: list[int], trees: list[tuple[list[int], list[int]]]) -> list[list[int]]:
+        """One verify pass over every row's tree of drafts: the new tokens of each row, those that decoding token by token would give
+        (greedy, or drawn with the same uniforms of the row's generator).  States and pages advance by the accepted path."""
+        rows = [([tok] + list(d), [-1] + [p + 1 for p in par], s.num_computed, s.slot, s.blocks.table, s.rope_delta)
+                for s, tok, (d, par) in zip(seqs, tokens, trees)]
+        self.model.verify_tree(rows)
+        if self._poll is not None:
+            self._poll()
+        temps = [s.params.temperature for s in seqs]
+        before = [self._generator(s).getstate() if t > 0 else None for s, t in zip(seqs, temps)]
+        us = [[self._generator(s).random() for _ in r[0]] if t > 0 else [] for s, t, r in zip(seqs, temps, rows)]
+        paths, last = self.model.accept_tree(temps, us)            # the read-back synchronises with the pass
+        if self._check is not None:
+            self._check()
+        self.model.commit_tree()
+        new_tokens = []
+        for s, row, path, tok, state in zip(seqs, rows, paths, last, before):
+            new = [int(row[0][j]) for j in path[1:]] + [int(tok)]
+            new_tokens.append(new)
+            if state is not None:                                  # one uniform a token, as if they had been drawn one by one
+                rng = self._generator(s)
+                rng.setstate(state)
+                for _ in new:
+                    rng.random()
+            if len(row[0]) > 1:
+                s.spec_steps += 1
+                s.spec_drafted += len(row[0]) - 1
+                s.spec_accepted += len(path) - 1
+                self.n_spec_drafted += len(row[0]) - 1
+                self.n_spec_accepted += len(path) - 1
+            s.blocks.commit(len(path))
+            s.num_computed += len(path)
+        self.n_decode_steps += 1
+        self.n_spec_steps += 1
+        return new_tokens
 
     SPEC_MAX_ROWS = 8
 
@@ -412,13 +484,14 @@ class ModelRunner:
             if greedy_tokens is not None:
                 return [int(v) for v in greedy_tokens[:len(seqs)].tolist()]
             return [int(v) for v in self.model.sample(logits, None, None).tolist()]
-        us = []
-        for s in seqs:
-            rng = self._rng.get(s.seq_id)
-            if rng is None:
-                rng = self._rng[s.seq_id] = random.Random(s.params.seed if s.params.seed is not None else s.seq_id)
-            us.append(rng.random())
+        us = [self._generator(s).random() for s in seqs]
         return [int(v) for v in self.model.sample(logits, temps, us).tolist()]
+
+    def _generator(self, seq: Sequence) -> random.Random:
+        rng = self._rng.get(seq.seq_id)
+        if rng is None:
+            rng = self._rng[seq.seq_id] = random.Random(seq.params.seed if seq.params.seed is not None else seq.seq_id)
+        return rng
 
     def forget(self, seq: Sequence) -> None:
         self._rng.pop(seq.seq_id, None)

@@ -42,6 +42,8 @@ def parser() -> argparse.ArgumentParser:
     ap.add_argument("--snapshot-interval", type=int, default=None)
     ap.add_argument("--spec-k", type=int, default=None)
     ap.add_argument("--spec-batch", action="store_true")
+    ap.add_argument("--spec-tree", type=int, default=None, help="drafted tokens a row may propose as a tree of continuations, up to --spec-k deep (0: one chain)")
+    ap.add_argument("--spec-sample", action="store_true", help="requests with a temperature draft too; the tokens are those of plain sampling")
     ap.add_argument("--spec-min-ctx", type=int, default=None,
                     help="rows with fewer cached tokens than this do not draft yet (0 = always)")
     ap.add_argument("--spec-sparse-k", type=int, default=0, help="approximate batched verify over the k best history blocks (refused when > 0: not built)")
@@ -87,6 +89,7 @@ def engine_config(args):
         max_seq=args.max_seq, quant=args.quant, kv_dtype=args.kv_dtype, prefix_cache=False if args.no_prefix_cache else None,
         num_blocks=args.num_blocks, snapshots=args.snapshots, snapshot_interval=args.snapshot_interval,
         spec_k=args.spec_k, spec_batch=True if args.spec_batch else None, spec_sparse_k=args.spec_sparse_k or None,
+        spec_tree=args.spec_tree, spec_sample=True if args.spec_sample else None,
         spec_min_ctx=args.spec_min_ctx, image_max_pixels=args.image_max_pixels, image_min_pixels=args.image_min_pixels,
         max_images=args.max_images, max_image_bytes=args.max_image_bytes, chunk=args.chunk,
         prefill_quantum=args.prefill_quantum, max_num_seqs=args.max_num_seqs,

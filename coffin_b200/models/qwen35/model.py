@@ -29,6 +29,7 @@ import torch
 
 from ...config import LINEAR, ModelConfig
 from ...ops import kernels as K
+from ...ops import tree
 from ...oracle import ops as O
 from ...weights.init import LM
 
@@ -1129,6 +1130,28 @@ class Qwen35Model:
         b["kv_slots"].copy_(h_kv)
         b["ridx"].copy_(h_ridx)
         dev_tables = [torch.tensor(t, dtype=torch.int32, device=self.device) for t in tables]
+
+        def linear(j, lw, proj, act):
+            K.gdn_decode(proj, lw.conv_w, lw.A_log, lw.dt_bias, lw.norm_w, self.ring[j], self.state[j], b["slot"],
+                         b["pos"], act, nk=c.linear_num_key_heads, nv=c.linear_num_value_heads,
+                         dk=c.linear_key_head_dim, dv=c.linear_value_head_dim, eps=self.eps, ntok=C,
+                         record=b["record"][j], write_state=False)
+
+        def full(j, lw, proj, act):
+            for i, (_tk, pos0, _s, _t, _d) in enumerate(rows):
+                sl = slice(i * C, (i + 1) * C)
+                K.attn_prefill(b["q"][sl], proj[sl], self.kpool[j], self.vpool[j], dev_tables[i], act[sl], q_pos0=pos0,
+                               nh=c.num_attention_heads, nkv=c.num_key_value_heads, hd=c.head_dim, **self._kvs(j))
+
+        self._verify_pass(b, N, linear, full)
+        self._verify_shape = (R, C, n)
+        return b["logits"].view(R, C, -1)[:n]
+
+    def _verify_pass(self, b: dict, N: int, linear, full) -> None:
+        """The layers over the ``N`` token rows staged in ``b``: norms, projections and feed-forward as in a decode step (up to
+        ``WIDE`` rows) or on the tcgen05 GEMM; ``linear`` / ``full`` run the mixer of a layer ``(index among its kind, weights, proj, act)``,
+        ``full`` with the queries in ``b["q"]`` and the rows' keys and values in the pools.  Logits go to ``b["logits"]``."""
+        c = self.cfg
         wide = N > WIDE
         cur, nxt = b["res"]
         K.embed_gather(self.embed, b["tokens"], cur)
@@ -1145,20 +1168,14 @@ class Qwen35Model:
             if lw.kind == LINEAR:
                 j = self.lin_ids[li]
                 act = b["act_lin"]
-                K.gdn_decode(proj, lw.conv_w, lw.A_log, lw.dt_bias, lw.norm_w, self.ring[j], self.state[j], b["slot"],
-                             b["pos"], act, nk=c.linear_num_key_heads, nv=c.linear_num_value_heads,
-                             dk=c.linear_key_head_dim, dv=c.linear_value_head_dim, eps=self.eps, ntok=C,
-                             record=b["record"][j], write_state=False)
+                linear(j, lw, proj, act)
             else:
                 j = self.full_ids[li]
                 act = b["act_full"]
                 K.attn_prep(proj, lw.qg, lw.kg, self.cos, self.sin, b["ridx"], b["kv_slots"], b["q"], self.kpool[j],
                             self.vpool[j], nh=c.num_attention_heads, nkv=c.num_key_value_heads, hd=c.head_dim,
                             rot=c.rotary_dim, eps=self.eps, **self._kvs(j))
-                for i, (_tk, pos0, _s, _t, _d) in enumerate(rows):
-                    sl = slice(i * C, (i + 1) * C)
-                    K.attn_prefill(b["q"][sl], proj[sl], self.kpool[j], self.vpool[j], dev_tables[i], act[sl], q_pos0=pos0,
-                                   nh=c.num_attention_heads, nkv=c.num_key_value_heads, hd=c.head_dim, **self._kvs(j))
+                full(j, lw, proj, act)
             if wide:
                 self._gemm(act, lw.w_out, out=cur, residual=cur)
                 K.rmsnorm(cur, lw.post_gain, self.eps, out=b["normed"])
@@ -1185,8 +1202,6 @@ class Qwen35Model:
         else:
             self._gemv(self.lm_head, None, b["logits"], norm=(cur, carry, self.final_gain, nxt, self.eps))
             b["final_res"] = nxt
-        self._verify_shape = (R, C, n)
-        return b["logits"].view(R, C, -1)[:n]
 
     def commit_batch(self, slots: list[int], steps: list[int]) -> None:
         """Apply, for row ``i`` of the last ``verify_batch`` call, its first ``steps[i]`` recorded
@@ -1219,6 +1234,105 @@ class Qwen35Model:
     def commit(self, slot: int, n_accept: int) -> None:
         """Apply the first ``n_accept`` recorded delta-net updates of the last one-sequence ``verify``."""
         self.commit_batch([slot], [n_accept])
+
+    # ------------------------------------------------------------------ trees of drafts
+    TREE_WIDTHS = (2, 4, 8, 16, 32, 64)
+
+    def _tree_buffers(self, R: int, C: int) -> dict:
+        b = self._verify_buffers(R, C)
+        if "anc" not in b:
+            c, dev = self.cfg, self.device
+            b["anc"] = torch.zeros(R, C, dtype=torch.int64, device=dev)
+            b["tables"] = torch.zeros(R, self.max_blocks_per_seq, dtype=torch.int32, device=dev)
+            b["raw"] = torch.zeros(len(self.lin_ids), R, C, c.lin_conv_dim, dtype=torch.bfloat16, device=dev)
+        return b
+
+    @torch.no_grad()
+    def verify_tree(self, rows: list[tuple]) -> torch.Tensor:
+        """Score a tree of drafted tokens behind each of ``R`` sequences in one pass over the weights.  ``rows[i] = (tokens, parents,
+        pos0, slot, block_table, rope_delta)``: node 0 is the last sampled token, a node's parent comes before it (the first one's is
+        -1), and a tree has at most ``C`` nodes, a width of ``TREE_WIDTHS`` with ``R * C <= 64``.  Returns logits ``[R, C, vocab]`` (anything
+        behind a tree's own nodes).  Node ``j`` keeps its key and value at position ``pos0 + j``; states are left untouched.
+        ``accept_tree`` and ``commit_tree`` follow."""
+        c = self.cfg
+        n = len(rows)
+        most = max(len(r[0]) for r in rows)
+        C = next((w for w in self.TREE_WIDTHS if w >= most), None)
+        if C is None or any(len(r[0]) != len(r[1]) or not r[0] for r in rows):
+            raise ValueError(f"trees of 1 to {self.TREE_WIDTHS[-1]} nodes with a parent each")
+        R = 1
+        while R < n:
+            R *= 2
+        N = R * C
+        if N > BUCKETS[-1]:
+            raise ValueError(f"{n} trees x {C} nodes exceed the {BUCKETS[-1]} token rows of one verify pass")
+        if self.tp is not None and (self.tp_world > 1 or self.ep_world > 1):
+            raise NotImplementedError("a verify pass over trees is single-GPU")
+        h_tok = torch.zeros(R, C, dtype=torch.int64)
+        h_anc = torch.zeros(R, C, dtype=torch.int64)
+        h_meta = torch.full((2, R), -1, dtype=torch.int32)             # slot, position
+        h_kv = torch.full((R, C), -1, dtype=torch.int32)
+        h_ridx = torch.zeros(R, C, dtype=torch.int32)
+        h_bt = torch.zeros(R, self.max_blocks_per_seq, dtype=torch.int32)
+        for i, (toks, parents, pos0, slot, table, delta) in enumerate(rows):
+            tl = table.tolist() if isinstance(table, torch.Tensor) else list(table)
+            self._check_row(pos0, len(toks), len(tl), delta, slot)
+            words = tree.path_words(parents)
+            if parents[0] != -1 or any(p < 0 for p in parents[1:]):
+                raise ValueError("node 0 is the only one without a parent")
+            k = len(toks)
+            h_tok[i, :k] = torch.tensor([int(x) for x in toks])
+            h_anc[i, :k] = torch.tensor(words)
+            h_meta[0, i], h_meta[1, i] = slot, pos0
+            h_kv[i, :k] = torch.tensor([tl[p // K.BLOCK] * K.BLOCK + p % K.BLOCK for p in range(pos0, pos0 + k)], dtype=torch.int32)
+            h_ridx[i, :k] = torch.tensor([pos0 + delta + (w & (1 << 64) - 1).bit_count() - 1 for w in words], dtype=torch.int32)
+            h_bt[i, :len(tl)] = torch.tensor(tl, dtype=torch.int32)
+        b = self._tree_buffers(R, C)
+        for name, h in (("tokens", h_tok.view(-1)), ("anc", h_anc), ("slot", h_meta[0]), ("pos", h_meta[1]), ("kv_slots", h_kv.view(-1)),
+                        ("ridx", h_ridx.view(-1)), ("tables", h_bt)):
+            b[name].copy_(h)
+        wide = max(len(r[4]) for r in rows)
+        tables = b["tables"][:, :wide]
+
+        def linear(j, lw, proj, act):
+            tree.gdn_tree(proj, lw.conv_w, lw.A_log, lw.dt_bias, lw.norm_w, self.ring[j], self.state[j], b["slot"], b["pos"], b["anc"], act,
+                          b["record"][j], b["raw"][j], nk=c.linear_num_key_heads, nv=c.linear_num_value_heads, dk=c.linear_key_head_dim,
+                          dv=c.linear_value_head_dim, eps=self.eps)
+
+        def full(j, lw, proj, act):
+            tree.attn_tree(b["q"], proj, self.kpool[j], self.vpool[j], tables, b["pos"], b["anc"], act, nh=c.num_attention_heads,
+                           nkv=c.num_key_value_heads, hd=c.head_dim, **self._kvs(j))
+
+        self._verify_pass(b, N, linear, full)
+        self._tree_shape = (R, C, n)
+        return b["logits"].view(R, C, -1)[:n]
+
+    @torch.no_grad()
+    def accept_tree(self, temps: list[float], us: list[list[float]]) -> tuple[list[list[int]], list[int]]:
+        """The paths that the sequences' own tokens take through the trees of the last ``verify_tree``: node lists from node 0 on, and
+        the token drawn at the end of each.  ``us[i]``: uniforms by depth (not looked at where ``temps[i] <= 0``, the arg-max)."""
+        R, C, n = self._tree_shape
+        b = self._tree_buffers(R, C)
+        h_t, h_u = torch.zeros(R), torch.zeros(R, C)
+        h_t[:n] = torch.tensor([float(t) for t in temps])
+        for i, u in enumerate(us):
+            h_u[i, :min(C, len(u))] = torch.tensor([float(x) for x in u[:C]])
+        path, steps, nxt = tree.verify_tree(b["logits"].view(R, C, -1), b["tokens"].view(R, C), b["anc"], h_t.to(self.device), h_u.to(self.device))
+        self._tree_path = path, steps
+        out = torch.cat([path.to(torch.int64), steps.to(torch.int64).view(R, 1), nxt.view(R, 1)], 1).tolist()       # one read-back
+        return [row[:row[C]] for row in out[:n]], [row[C + 1] for row in out[:n]]
+
+    @torch.no_grad()
+    def commit_tree(self) -> None:
+        """Make the paths of the last ``accept_tree`` part of their sequences: keys and values to consecutive positions, states and
+        convolution rings advanced."""
+        R, C, _n = self._tree_shape
+        b = self._tree_buffers(R, C)
+        path, steps = self._tree_path
+        if self.full_ids:
+            tree.kv_tree_commit(self.kpool, self.vpool, b["tables"], b["pos"], path, steps, self.kscale, self.vscale)
+        if self.lin_ids:
+            tree.gdn_tree_commit(self.state, self.ring, b["record"], b["raw"], b["slot"], b["pos"], path, steps)
 
     # ------------------------------------------------------------------ runner hooks
     def poll_status(self) -> None:

@@ -240,6 +240,39 @@ class OracleEngineModel:
                 cos, sin = O.mrope_cos_sin(pos.reshape(1, -1).expand(3, -1), c.rotary_dim, c.rope_theta, c.mrope_section)
                 self._forward(self.embed_tokens(torch.tensor(tokens[:n_accept])), pos0, slot, table, cos, sin)
 
+    @torch.no_grad()
+    def verify_tree(self, rows: list[tuple]) -> torch.Tensor:
+        """Logits ``[R, C, vocab]`` of trees of drafted tokens ``(tokens, parents, pos0, slot, block_table, rope_delta)``: the twin runs
+        every node's path from the sequence's own state.  States are left as they were; ``accept_tree`` and ``commit_tree`` follow."""
+        c = self.cfg
+        out = torch.zeros(len(rows), max(len(r[0]) for r in rows), c.vocab_size)
+        self._tree = []
+        for i, (tokens, parents, pos0, slot, block_table, rope_delta) in enumerate(rows):
+            table = block_table.clone() if isinstance(block_table, torch.Tensor) else torch.tensor(list(block_table), dtype=torch.int32)
+            snap = self.snapshot_state(slot)
+            for j in range(len(tokens)):
+                path = [j]
+                while parents[path[0]] >= 0:
+                    path.insert(0, parents[path[0]])
+                pos = torch.arange(pos0, pos0 + len(path)) + rope_delta
+                cos, sin = O.mrope_cos_sin(pos.reshape(1, -1).expand(3, -1), c.rotary_dim, c.rope_theta, c.mrope_section)
+                x = self._forward(self.embed_tokens(torch.tensor([tokens[k] for k in path])), pos0, slot, table, cos, sin)
+                out[i, j] = self._head(x[-1:])[0]
+                self.restore_state(slot, snap)
+            self._tree.append((list(tokens), list(parents), pos0, table, rope_delta, snap, slot, out[i]))
+        return out
+
+    def accept_tree(self, temps: list[float], us: list[list[float]]) -> tuple[list[list[int]], list[int]]:
+        picked = [O.tree_walk(lg, toks, parents, t, u) for (toks, parents, _p, _b, _d, _s, _l, lg), t, u in zip(self._tree, temps, us)]
+        self._tree_paths = [p for p, _t in picked]
+        return self._tree_paths, [t for _p, t in picked]
+
+    @torch.no_grad()
+    def commit_tree(self) -> None:
+        self._verify = [([toks[j] for j in path], pos0, table, delta, snap, slot)
+                        for (toks, _p, pos0, table, delta, snap, slot, _l), path in zip(self._tree, self._tree_paths)]
+        self.commit_batch([v[5] for v in self._verify], [len(v[0]) for v in self._verify])
+
     def verify(self, tokens: list[int], pos0: int, slot: int, block_table: torch.Tensor, rope_delta: int = 0) -> torch.Tensor:
         return self.verify_batch([(tokens, pos0, slot, block_table, rope_delta)])[0]
 
@@ -256,7 +289,5 @@ class OracleEngineModel:
             if t <= 0:
                 out.append(int(logits[i].argmax()))
                 continue
-            cdf = torch.softmax(logits[i].double() / t, -1).cumsum(0)
-            idx = int(torch.searchsorted(cdf, torch.tensor(u * float(cdf[-1]), dtype=torch.float64), right=True))
-            out.append(min(idx, logits.shape[1] - 1))
+            out.append(O.draw(logits[i], t, u))
         return torch.tensor(out)

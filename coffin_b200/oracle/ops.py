@@ -213,6 +213,28 @@ def delta_commit(base: torch.Tensor, rec_k, rec_d, rec_alpha, steps: int) -> tor
     return st
 
 
+# ---------------------------------------------------------------- sampling
+def draw(logits: torch.Tensor, temperature: float, u: float) -> int:
+    """Inverse-CDF draw from ``softmax(logits / temperature)`` in 64 bits; the arg-max where the temperature is not positive."""
+    if temperature <= 0:
+        return int(logits.argmax())
+    cdf = torch.softmax(logits.double() / temperature, -1).cumsum(0)
+    at = int(torch.searchsorted(cdf, torch.tensor(u * float(cdf[-1]), dtype=torch.float64), right=True))
+    return min(at, logits.shape[-1] - 1)
+
+
+def tree_walk(logits: torch.Tensor, tokens, parents, temperature: float, us) -> tuple[list[int], int]:
+    """Path from node 0 through the children that carry the token drawn at each node (``us`` by depth), and the token drawn at its
+    end: what sampling token by token with the same uniforms gives.  ``logits [C, vocab]``."""
+    path = [0]
+    while True:
+        t = draw(logits[path[-1]], temperature, us[len(path) - 1] if temperature > 0 else 0.0)
+        nxt = [j for j, p in enumerate(parents) if p == path[-1] and tokens[j] == t]
+        if not nxt:
+            return path, t
+        path.append(nxt[0])
+
+
 # ---------------------------------------------------------------- MoE
 def moe_route(logits: torch.Tensor, top_k: int, normalize: bool = True):
     """fp32 softmax -> top-k -> optional renormalisation. Returns ``(index, weight)``."""

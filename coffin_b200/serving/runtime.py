@@ -267,7 +267,7 @@ class Server:
                 "prefill_ms": round(prefill_ms, 2), "decode_ms": round(decode_ms, 2),
                 "decode_tok_s": round((n_new - 1) / (decode_ms / 1e3), 2) if decode_ms > 0 and n_new > 1 else 0.0,
                 "stopped": seq.finish_reason,
-                "spec_k": self.engine.runner.spec_k_of(seq) if seq.params.temperature <= 0 else 0,
+                "spec_k": self.engine.runner.spec_k_of(seq),
                 "spec": ({"steps": seq.spec_steps, "drafted": seq.spec_drafted, "accepted": seq.spec_accepted,
                           "accept_rate": round(seq.spec_accepted / seq.spec_drafted, 4) if seq.spec_drafted else 0.0}
                          if seq.spec_steps else None)}
