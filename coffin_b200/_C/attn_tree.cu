@@ -590,35 +590,26 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   }
 }
 
-// EPL channels of one lane of a pool row, as floats (codes unscaled)
-template <int EPL, bool Q8>
-__device__ __forceinline__ void row_piece(const void* pool, int64_t at, float* x) {
-  if (Q8) {
-    const int8_t* p = (const int8_t*)pool + at;
-    if (EPL == 8) {
-      const uint2 w = *reinterpret_cast<const uint2*>(p);
-#pragma unroll
-      for (int e = 0; e < EPL; ++e) x[e] = (float)(int8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)) & 0xff);
-    } else {
-#pragma unroll
-      for (int e = 0; e < EPL; ++e) x[e] = (float)p[e];
-    }
-  } else {
-    const bf16* p = (const bf16*)pool + at;
-    if (EPL == 8) bf16x8_to_float(*reinterpret_cast<const uint4*>(p), x);
-    else {
-#pragma unroll
-      for (int e = 0; e < EPL; e += 2) {
-        const float2 f = __bfloat1622float2(*reinterpret_cast<const bf162*>(p + e));
-        x[e] = f.x; x[e + 1] = f.y;
-      }
-    }
+// EPL channels of one lane of a row, packed as they lie in memory (words of two bf16 or of four codes), and as floats (codes unscaled)
+template <int EPL, bool Q8> struct RowPiece {
+  static constexpr int W = Q8 ? (EPL + 3) / 4 : EPL / 2;
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const void* pool, int64_t at) {
+    const char* p = (const char*)pool + at * (Q8 ? 1 : 2);
+    if (W == 4) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(p);
+    else if (W == 2) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(p);
+    else if (Q8 && EPL == 2) w[0] = *reinterpret_cast<const uint16_t*>(p);
+    else w[0] = *reinterpret_cast<const uint32_t*>(p);
   }
-}
+  __device__ __forceinline__ float at(int e) const {
+    if (Q8) return (float)(int8_t)(w[e / 4] >> (8 * (e & 3)) & 0xff);
+    return __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+  }
+};
 
 // A warp a (node, head): the node's path, the partial sums of the cache, the gate and the store.  Lanes own hd / 32 channels of a row;
-// lane i also keeps slot and score of nodes i and i + 32, and the maximum and sum of a partial.  Latency is all there is to it: tables,
-// scores and maxima are fetched by all lanes at once, rows four at a time.
+// lane i also keeps the pool rows of nodes i and i + 32, and the maximum and sum of a partial.  Latency is all there is to it: tables and
+// maxima are fetched by all lanes at once, keys and values of four nodes together, partials four at a time.
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) {
   constexpr int EPL = HD / 32;
@@ -634,14 +625,15 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
   on = (on & (~0ull >> (63 - j))) | 1ull << j;              // a path ends at its node
   const int kvh = h / a.rep;
   const int64_t row = (int64_t)r * a.C + j;
-  float q[EPL], o[EPL], gate[EPL];
-  row_piece<EPL, false>(a.q, (row * a.nh + h) * HD + lane * EPL, q);
+  float q[EPL], o[EPL];
+  RowPiece<EPL, false> qp, gp;
+  qp.load(a.q, (row * a.nh + h) * HD + lane * EPL);
+  if (a.gate) gp.load(a.gate, row * a.ldg + (int64_t)h * 2 * HD + HD + lane * EPL);
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) { q[e] *= a.scale_log2; o[e] = 0.f; gate[e] = 0.f; }
-  if (a.gate) row_piece<EPL, false>(a.gate, row * a.ldg + (int64_t)h * 2 * HD + HD + lane * EPL, gate);
+  for (int e = 0; e < EPL; ++e) { q[e] = qp.at(e) * a.scale_log2; o[e] = 0.f; }
   // pool rows of the path; a page that is none takes its nodes off it
   int64_t kr[2];
-  float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f}, sc[2] = {-INFINITY, -INFINITY};
+  float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
   uint64_t path = 0;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -663,67 +655,65 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
     b0 = piece_of(g0, T, G);
     parts = piece_of(g0 + n - 1, T, G) - b0 + 1;
   }
-  float m = -INFINITY;
+  const int64_t at0 = (int64_t)(b0 + item) * a.used + lrow % kRows;
+  float m = -INFINITY, l = 0.f;
 #pragma unroll 1
-  for (int b = lane; b < parts; b += 32) m = fmaxf(m, a.part_ml[((int64_t)(b0 + b + item) * a.used + lrow % kRows) * 2]);
-  // scores of the path
-  auto take = [&](uint64_t& rest) {                         // next node, -1: none left
-    const int i = rest ? __ffsll((long long)rest) - 1 : -1;
-    rest &= rest - 1;
-    return i;
-  };
+  for (int b = lane; b < parts; b += 32) m = fmaxf(m, a.part_ml[(at0 + (int64_t)b * a.used) * 2]);
+  m = warp_max(m);
+  // the path, four nodes at a time: keys and values are requested together
 #pragma unroll 1
   for (uint64_t rest = path; rest;) {
-    int id[4];
-    float s[4];
+    RowPiece<EPL, Q8> kp[4], vp[4];
+    float s[4], kf[4], vf[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      id[k] = take(rest);
-      const int64_t at = id[k] < 32 ? __shfl_sync(0xffffffffu, kr[0], id[k] & 31) : __shfl_sync(0xffffffffu, kr[1], id[k] & 31);
-      float x[EPL];
-      s[k] = 0.f;
-      if (id[k] >= 0) {
-        row_piece<EPL, Q8>(a.kpool, at * HD + lane * EPL, x);
-#pragma unroll
-        for (int e = 0; e < EPL; ++e) s[k] = fmaf(q[e], x[e], s[k]);
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      s[k] = warp_sum(s[k]);
-      if (id[k] == lane) sc[0] = s[k] * ks[0];
-      if (id[k] == lane + 32) sc[1] = s[k] * ks[1];
-    }
-  }
-  m = warp_max(fmaxf(m, fmaxf(sc[0], sc[1])));
-  const float ms = m == -INFINITY ? 0.f : m;
-  float w[2] = {exp2f(sc[0] - ms), exp2f(sc[1] - ms)}, l = w[0] + w[1];
-  w[0] *= vs[0]; w[1] *= vs[1];
-#pragma unroll 1
-  for (uint64_t rest = path; rest;) {
-    float x[4][EPL], f[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int i = take(rest);
+      const int i = rest ? __ffsll((long long)rest) - 1 : -1;
+      rest &= rest - 1;
       const int64_t at = i < 32 ? __shfl_sync(0xffffffffu, kr[0], i & 31) : __shfl_sync(0xffffffffu, kr[1], i & 31);
-      f[k] = i < 32 ? __shfl_sync(0xffffffffu, w[0], i & 31) : __shfl_sync(0xffffffffu, w[1], i & 31);
-      if (i >= 0) row_piece<EPL, Q8>(a.vpool, at * HD + lane * EPL, x[k]);
-      else {
-        f[k] = 0.f;
+      kf[k] = vf[k] = 1.f;
+      if (Q8) {
+        kf[k] = i < 32 ? __shfl_sync(0xffffffffu, ks[0], i & 31) : __shfl_sync(0xffffffffu, ks[1], i & 31);
+        vf[k] = i < 32 ? __shfl_sync(0xffffffffu, vs[0], i & 31) : __shfl_sync(0xffffffffu, vs[1], i & 31);
+      }
+      s[k] = i >= 0 ? 0.f : -INFINITY;
+      if (i >= 0) {
+        kp[k].load(a.kpool, at * HD + lane * EPL);
+        vp[k].load(a.vpool, at * HD + lane * EPL);
+      } else {
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) x[k][e] = 0.f;
+        for (int x = 0; x < RowPiece<EPL, Q8>::W; ++x) vp[k].w[x] = 0u;
       }
     }
+    float mn = m;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
+    for (int k = 0; k < 4; ++k) {
+      if (s[k] == 0.f) {                                    // a node (the same for the warp)
+        float d = 0.f;
 #pragma unroll
-      for (int e = 0; e < EPL; ++e) o[e] = fmaf(f[k], x[k][e], o[e]);
+        for (int e = 0; e < EPL; ++e) d = fmaf(q[e], kp[k].at(e), d);
+        s[k] = warp_sum(d) * kf[k];
+      }
+      mn = fmaxf(mn, s[k]);
+    }
+    const float ms = mn == -INFINITY ? 0.f : mn, c = exp2f(m - ms);
+    m = mn;
+    l *= c;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) o[e] *= c;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float w = exp2f(s[k] - ms);
+      if (lane == 0) l += w;                                // the partials' sums are one a lane
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[e] = fmaf(w * vf[k], vp[k].at(e), o[e]);
+    }
   }
+  const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
   for (int c = 0; c < parts; c += 32) {
     float f = 0.f;
     if (c + lane < parts) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + ((int64_t)(b0 + c + lane + item) * a.used + lrow % kRows) * 2);
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (at0 + (int64_t)(c + lane) * a.used) * 2);
       f = exp2f(ml.x - ms);                                 // 0 where these pages hold no key
       l += f * ml.y;
     }
@@ -734,31 +724,29 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         g[k] = __shfl_sync(0xffffffffu, f, (b + k) & 31);
-        const bool in = b + k < here;
-        const float* po = a.part_o + ((int64_t)(b0 + c + b + k + item) * a.used + lrow % kRows) * HD + lane * EPL;
+        const float* po = a.part_o + (at0 + (int64_t)(c + min(b + k, here - 1)) * a.used) * HD + lane * EPL;
+        if (b + k >= here) g[k] = 0.f;                      // the last one once more, with no weight
+        if (EPL == 8) {
+          *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(po);
+          *reinterpret_cast<float4*>(x[k] + EPL / 2) = *reinterpret_cast<const float4*>(po + 4);
+        } else {
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) x[k][e] = 0.f;
-        if (in) {
-          if (EPL == 8) {
-            *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(po);
-            *reinterpret_cast<float4*>(x[k] + EPL / 2) = *reinterpret_cast<const float4*>(po + 4);
-          } else {
-#pragma unroll
-            for (int e = 0; e < EPL; ++e) x[k][e] = po[e];
-          }
-        } else g[k] = 0.f;
+          for (int e = 0; e < EPL; ++e) x[k][e] = po[e];
+        }
       }
 #pragma unroll
       for (int k = 0; k < 4; ++k)
+        if (g[k] != 0.f) {
 #pragma unroll
-        for (int e = 0; e < EPL; ++e) o[e] = fmaf(g[k], x[k][e], o[e]);
+          for (int e = 0; e < EPL; ++e) o[e] = fmaf(g[k], x[k][e], o[e]);
+        }
     }
   }
   l = warp_sum(l);
   const float inv = l > 0.f ? 1.f / l : 0.f;
   bf16* op = a.out + row * a.ldo + (int64_t)h * HD + lane * EPL;
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) o[e] *= inv * (a.gate ? sigmoid_f(gate[e]) : 1.f);
+  for (int e = 0; e < EPL; ++e) o[e] *= inv * (a.gate ? sigmoid_f(gp.at(e)) : 1.f);
   if (EPL == 8) *reinterpret_cast<uint4*>(op) = float_to_bf16x8(o);
   else {
 #pragma unroll
