@@ -764,9 +764,13 @@ int launch_tree(const TreeAttnArgs& a, int64_t slots, cudaStream_t st) {
   }
   const size_t smem = TreeRing<HD, Q8>::bytes;
   auto kern = tree_cache_kernel<HD, Q8>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
-  e = cb_launch(kern, dim3((unsigned)a.ctas), dim3(Q8 ? 352 + kLoaders : 352), smem, st, tmK, tmV, a);
+  static SmemLimit limit;
+  cudaError_t e;
+  {
+    std::lock_guard<std::mutex> lock(limit.held);
+    e = limit.set(kern, smem);
+    if (e == cudaSuccess) e = cb_launch(kern, dim3((unsigned)a.ctas), dim3(Q8 ? 352 + kLoaders : 352), smem, st, tmK, tmV, a);
+  }
   if (e != cudaSuccess) return (int)e;
   const int64_t tasks = (int64_t)a.R * a.C * a.nh;
   return (int)cb_launch(tree_finish_kernel<HD, Q8>, dim3((unsigned)((tasks + 7) / 8)), dim3(256), 0, st, a);

@@ -14,8 +14,9 @@
 //
 // 1. row_stats: the logits are read once; a warp a (part of the vocabulary, row) leaves the part's maximum, its first place and the sum of
 //    exp((x - maximum) / T).
-// 2. tree_pick / draft_rest: a draw needs its part of the row once more (draws from max(p - q, 0) the whole row of the node they end at).
-// 3. tree_walk / draft_pick: the path and the token after it.
+// 2. tree_pick: a draw needs its part of its row once more; the last CTA of a sequence to arrive walks the tree.
+//    draft_rest: draws from max(p - q, 0) need the whole row at which the chain ends; the last CTA of a sequence draws.
+// The arrivals are counted in workspace that the first kernel clears.
 #include <algorithm>
 
 #include "common.cuh"
@@ -40,6 +41,7 @@ struct VerifyArgs {
   PartStat* stats;                            // [R * C, P]
   int* picks;                                 // tree: [R * C]
   double2* rest;                              // chain: [R, P] sums of max(p - q, 0) and of p
+  unsigned* arrived;                          // [R]
   int* path; int* steps; int64_t* next;
   int64_t V, per;
   int R, C, P;
@@ -123,6 +125,7 @@ __global__ void __launch_bounds__(kNT) row_stats_kernel(const VerifyArgs a) {
   griddep_wait();
   const int lane = threadIdx.x & 31, p = blockIdx.x * (kNT / 32) + (threadIdx.x >> 5), r = blockIdx.y / a.C, j = blockIdx.y % a.C;
   roots[threadIdx.x] = kRoots[0][threadIdx.x / 16] * kRoots[1][threadIdx.x % 16];
+  if (p == 0 && j == 0 && lane == 0) a.arrived[r] = 0;
   __syncthreads();
   if (p >= a.P || !row_used(a, r, j)) return;
   const float* row = a.logits + r * a.lds + j * a.ldr;
@@ -284,49 +287,62 @@ struct RowWeights {                  // exp((logit - mx) / T)
   __device__ __forceinline__ double one(int64_t at) const { return weight(row[at], mx, s256); }
 };
 
-// A node's own token.
-__global__ void __launch_bounds__(kNT) tree_pick_kernel(const VerifyArgs a) {
+// Whether this CTA is the last of `all` to arrive for sequence r; what the others have written before is visible to it then.
+__device__ __forceinline__ bool last_of(const VerifyArgs& a, int r, unsigned all) {
+  __shared__ bool last;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(a.arrived + r, 1u) == all - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  return last;
+}
+
+__device__ __forceinline__ void tree_walk(const VerifyArgs& a, int r);
+
+// A node's own token (thread 0's).
+__device__ __forceinline__ int node_token(const VerifyArgs& a, int r, int j) {
   __shared__ double red[kNT / 32];
-  double before;
-  griddep_launch();
-  griddep_wait();
-  const int r = blockIdx.x / a.C, j = blockIdx.x % a.C;
-  if (!row_used(a, r, j)) return;
-  const PartStat* st = a.stats + (int64_t)blockIdx.x * a.P;
+  const PartStat* st = a.stats + ((int64_t)r * a.C + j) * a.P;
   const float T = a.temperature[r];
   float mx;
   int arg;
-  double total;
+  double total, whole, before;
   row_whole(st, a.P, T, mx, arg, total);
-  if (!(T > 0.f) || !(total > 0.0)) {
-    if (threadIdx.x == 0) a.picks[blockIdx.x] = arg < a.V ? arg : 0;
-    return;
-  }
+  if (!(T > 0.f) || !(total > 0.0)) return arg < a.V ? arg : 0;
   const double s256 = scale256(T);
-  const int depth = __popcll((uint64_t)a.anc[(int64_t)r * a.C + j] & ~(~0ull << j));
-  const int p = threadIdx.x;
-  const double mine = p < a.P ? st[p].sum * weight(st[p].mx, mx, s256) : 0.0;
-  double whole;
-  const double incl = block_scan_d<kNT>(mine, red, &whole);
+  const int depth = __popcll((uint64_t)a.anc[(int64_t)r * a.C + j] & ~(~0ull << j)), p = threadIdx.x;
+  const double mine = p < a.P ? st[p].sum * weight(st[p].mx, mx, s256) : 0.0, incl = block_scan_d<kNT>(mine, red, &whole);
   const double target = (double)a.u[(int64_t)r * a.C + depth] * whole;
   const int part = pick_part(mine, incl, target, &before);
   const float* row = a.logits + r * a.lds + j * a.ldr;
   const int64_t b = part * a.per, pick = pick_range(RowWeights{row, ((uintptr_t)row & 15) == 0, mx, s256}, b, min(a.V, b + a.per), before, target);
-  if (threadIdx.x == 0) a.picks[blockIdx.x] = pick < 0 ? arg : (int)pick;
+  return pick < 0 ? arg : (int)pick;
+}
+
+__global__ void __launch_bounds__(kNT) tree_pick_kernel(const VerifyArgs a) {
+  griddep_launch();
+  griddep_wait();
+  const int r = blockIdx.x / a.C, j = blockIdx.x % a.C;
+  if (row_used(a, r, j)) {
+    const int token = node_token(a, r, j);
+    if (threadIdx.x == 0) a.picks[blockIdx.x] = token;
+  }
+  if (last_of(a, r, a.C)) tree_walk(a, r);
 }
 
 // Node 0, then the first child that carries the token drawn at the node reached; children come after their parents.
-__global__ void __launch_bounds__(kNodes) tree_walk_kernel(const VerifyArgs a) {
+__device__ __forceinline__ void tree_walk(const VerifyArgs& a, int r) {
   __shared__ int parent[kNodes];
   __shared__ int64_t token[kNodes], pick[kNodes];
-  griddep_launch();
-  griddep_wait();
-  const int r = blockIdx.x, j = threadIdx.x;
+  const int j = threadIdx.x;
   if (j < a.C) {
     const uint64_t on = (uint64_t)a.anc[(int64_t)r * a.C + j], up = on & ~(~0ull << j);
     parent[j] = on != 0 && up != 0 ? 63 - __clzll((long long)up) : -1;
     token[j] = a.tokens[(int64_t)r * a.C + j];
-    pick[j] = on != 0 ? a.picks[(int64_t)r * a.C + j] : -1;
+    pick[j] = on != 0 ? __ldcg(a.picks + (int64_t)r * a.C + j) : -1;
     a.path[(int64_t)r * a.C + j] = -1;
   }
   __syncthreads();
@@ -335,6 +351,7 @@ __global__ void __launch_bounds__(kNodes) tree_walk_kernel(const VerifyArgs a) {
   if (pick[0] >= 0) {
     a.path[(int64_t)r * a.C] = 0;
     n = 1;
+#pragma unroll 1
     for (int i = 1; i < a.C; ++i)
       if (parent[i] == cur && token[i] == pick[cur]) {
         a.path[(int64_t)r * a.C + n++] = i;
@@ -428,14 +445,22 @@ __global__ void __launch_bounds__(kNT) draft_rest_kernel(const VerifyArgs a) {
   __shared__ double red[2][kNT / 32];
   griddep_launch();
   griddep_wait();
-  const int p = blockIdx.x, r = blockIdx.y, n = min(a.lengths[r], a.C);
-  if (n < 1 || !(a.temperature[r] > 0.f)) return;
+  const int p = blockIdx.x, r = blockIdx.y, n = min(a.lengths[r], a.C), tid = threadIdx.x;
+  if (n < 1) {
+    if (p == 0 && tid == 0) { a.steps[r] = 0; a.next[r] = -1; }
+    return;
+  }
   const ChainEnd c = chain_end<kNT>(a, r, n);
-  const RestWeights w = rest_weights(a, r, n, c);
+  if (p == 0 && tid == 0) a.steps[r] = c.at + 1;
+  if (!(a.temperature[r] > 0.f) || !(c.total > 0.0)) {
+    if (p == 0 && tid == 0) a.next[r] = c.arg < a.V ? c.arg : 0;
+    return;
+  }
+  RestWeights w = rest_weights(a, r, n, c);
   const int64_t b = p * a.per, e = min(a.V, b + a.per);
   double rest = 0.0, all = 0.0;
 #pragma unroll 1
-  for (int64_t at = b + threadIdx.x * kPE; at < e; at += kNT * kPE) {
+  for (int64_t at = b + tid * kPE; at < e; at += kNT * kPE) {
     double x[kPE], y[kPE];
     w.both(at, e, x, y);
 #pragma unroll
@@ -443,46 +468,26 @@ __global__ void __launch_bounds__(kNT) draft_rest_kernel(const VerifyArgs a) {
   }
   rest = warp_sum_d(rest);
   all = warp_sum_d(all);
-  if ((threadIdx.x & 31) == 0) { red[0][threadIdx.x >> 5] = rest; red[1][threadIdx.x >> 5] = all; }
+  if ((tid & 31) == 0) { red[0][tid >> 5] = rest; red[1][tid >> 5] = all; }
   __syncthreads();
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     rest = all = 0.0;
     for (int i = 0; i < kNT / 32; ++i) { rest += red[0][i]; all += red[1][i]; }
     a.rest[(int64_t)r * a.P + p] = make_double2(rest, all);
   }
-}
-
-__global__ void __launch_bounds__(kNT) draft_pick_kernel(const VerifyArgs a) {
-  __shared__ double red[kNT / 32];
-  double before;
-  griddep_launch();
-  griddep_wait();
-  const int r = blockIdx.x, n = min(a.lengths[r], a.C), p = threadIdx.x;
-  if (n < 1) {
-    if (p == 0) { a.steps[r] = 0; a.next[r] = -1; }
-    return;
-  }
-  const ChainEnd c = chain_end<kNT>(a, r, n);
-  if (p == 0) a.steps[r] = c.at + 1;
-  if (!(a.temperature[r] > 0.f) || !(c.total > 0.0)) {
-    if (p == 0) a.next[r] = c.arg < a.V ? c.arg : 0;
-    return;
-  }
-  const double2 mine2 = p < a.P ? a.rest[(int64_t)r * a.P + p] : make_double2(0.0, 0.0);
-  double whole;
-  double incl = block_scan_d<kNT>(mine2.x, red, &whole);
-  const bool rest = whole > 0.0;                  // nothing left over: drafts drawn from q are always kept then, up to rounding
-  double mine = mine2.x;
-  if (!rest) {
+  if (!last_of(a, r, a.P)) return;
+  const double2 mine2 = tid < a.P ? __ldcg(a.rest + (int64_t)r * a.P + tid) : make_double2(0.0, 0.0);
+  double whole, before;
+  double incl = block_scan_d<kNT>(mine2.x, red[0], &whole), mine = mine2.x;
+  w.rest = whole > 0.0;                           // nothing left over: drafts drawn from q are always kept then, up to rounding
+  if (!w.rest) {
     mine = mine2.y;
-    incl = block_scan_d<kNT>(mine, red, &whole);
+    incl = block_scan_d<kNT>(mine, red[0], &whole);
   }
   const double target = (double)a.u_draw[r] * whole;
   const int part = pick_part(mine, incl, target, &before);
-  RestWeights w = rest_weights(a, r, n, c);
-  w.rest = rest;
-  const int64_t b = part * a.per, pick = pick_range(w, b, min(a.V, b + a.per), before, target);
-  if (p == 0) a.next[r] = pick < 0 ? c.arg : pick;
+  const int64_t b1 = part * a.per, pick = pick_range(w, b1, min(a.V, b1 + a.per), before, target);
+  if (tid == 0) a.next[r] = pick < 0 ? c.arg : pick;
 }
 
 // Logits of a part: two steps of a warp where there are few rows, four where there are enough warps without; more where a row would have
@@ -499,7 +504,7 @@ int parts_of(int64_t rows, int64_t V, int64_t* per) {
 CB_EXPORT int64_t cb_verify_scratch(int64_t R, int64_t C, int64_t V) {
   int64_t per;
   const int64_t P = parts_of(R * C, V, &per);
-  return R * C * P * (int64_t)sizeof(PartStat) + R * P * (int64_t)sizeof(double2) + R * C * (int64_t)sizeof(int);
+  return R * C * P * (int64_t)sizeof(PartStat) + R * P * (int64_t)sizeof(double2) + R * C * (int64_t)sizeof(int) + R * (int64_t)sizeof(unsigned);
 }
 
 CB_EXPORT int cb_verify_tree(const void* logits, int64_t lds, int64_t ldr, const void* tokens, const void* anc, const void* temperature,
@@ -512,10 +517,10 @@ CB_EXPORT int cb_verify_tree(const void* logits, int64_t lds, int64_t ldr, const
   a.V = V; a.R = (int)R; a.C = (int)C; a.P = parts_of(R * C, V, &a.per);
   a.stats = (PartStat*)scratch;
   a.picks = (int*)(a.stats + R * C * a.P);
+  a.arrived = (unsigned*)(a.picks + R * C);
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e = cb_launch(row_stats_kernel, dim3((unsigned)((a.P + kNT / 32 - 1) / (kNT / 32)), (unsigned)(R * C)), dim3(kNT), 0, st, a);
   if (e == cudaSuccess) e = cb_launch(tree_pick_kernel, dim3((unsigned)(R * C)), dim3(kNT), 0, st, a);
-  if (e == cudaSuccess) e = cb_launch(tree_walk_kernel, dim3((unsigned)R), dim3(kNodes), 0, st, a);
   return (int)e;
 }
 
@@ -531,9 +536,9 @@ CB_EXPORT int cb_verify_drafts(const void* logits, int64_t lds, int64_t ldr, con
   a.V = V; a.R = (int)R; a.C = (int)C; a.P = parts_of(R * C, V, &a.per);
   a.stats = (PartStat*)scratch;
   a.rest = (double2*)(a.stats + R * C * a.P);
+  a.arrived = (unsigned*)(a.rest + R * a.P);
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e = cb_launch(row_stats_kernel, dim3((unsigned)((a.P + kNT / 32 - 1) / (kNT / 32)), (unsigned)(R * C)), dim3(kNT), 0, st, a);
   if (e == cudaSuccess) e = cb_launch(draft_rest_kernel, dim3((unsigned)a.P, (unsigned)R), dim3(kNT), 0, st, a);
-  if (e == cudaSuccess) e = cb_launch(draft_pick_kernel, dim3((unsigned)R), dim3(kNT), 0, st, a);
   return (int)e;
 }

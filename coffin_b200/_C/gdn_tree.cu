@@ -110,7 +110,9 @@ struct TreeState {
   static constexpr int WC = DVS / 32, SL = WC == 4 ? 8 : 4, VG = kThreads / 32 / SL, KR = DK / SL, BV = WC == 4 ? 8 : 32;
 };
 
-template <int DK, int DVS>
+// With many nodes and a whole head a CTA, tiles of eight vectors by eight columns a thread from shared memory are the better way: no partial
+// products, and 16 multiplications for a load of 16 bytes.  (192 heads of 64 nodes 106.7 -> 94.5 us, of 48 nodes 76.5 -> 75.1, 240 heads of 40 nodes 67.0 -> 69.9.)
+template <int DK, int DVS, bool TILE>
 struct TreeSmem {                         // floats
   static constexpr int LK = DK + 4;       // rows a quarter warp reads lie in different banks
   int kn, qn, d, o, z, P, A, B, D, total; // z as bf16; A, B, D (and the doubling's scratch in D's place) follow the partial products in their place
@@ -125,7 +127,7 @@ struct TreeSmem {                         // floats
     D = B + Cp * (Cp + 4);
     const int scratch = Cp * DVS > 32 * 36 ? Cp * DVS : 32 * 36;
     const int bv = 2 * Cp < TreeState<DK, DVS>::BV ? 2 * Cp : TreeState<DK, DVS>::BV;
-    const int a = P + TreeState<DK, DVS>::SL * bv * DVS, b = D + scratch;
+    const int a = P + (TILE ? DK * DVS : TreeState<DK, DVS>::SL * bv * DVS), b = D + scratch;
     total = a > b ? a : b;
   }
 };
@@ -161,9 +163,9 @@ __device__ __forceinline__ void sync_all() {
   else __syncthreads();
 }
 
-template <int DK, int DV, int DVS>
+template <int DK, int DV, int DVS, bool TILE>
 __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a) {
-  constexpr int NS = DV / DVS, LK = TreeSmem<DK, DVS>::LK;
+  constexpr int NS = DV / DVS, LK = TreeSmem<DK, DVS, TILE>::LK;
   extern __shared__ __align__(16) float sm[];
   __shared__ uint64_t anc_s[kMaxNodes];
   __shared__ double c_s[kMaxNodes];
@@ -173,7 +175,7 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a)
   griddep_wait();
   const int cg = blockIdx.x, h = blockIdx.y, r = blockIdx.z, kh = h / a.rep, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int C = a.C, Cp = a.Cp, LA = Cp + 4, heads = 2 * a.nk + a.nv;
-  const TreeSmem<DK, DVS> off(Cp);
+  const TreeSmem<DK, DVS, TILE> off(Cp);
   float *kn = sm + off.kn, *qn = sm + off.qn, *d = sm + off.d, *o = sm + off.o, *A = sm + off.A, *B = sm + off.B, *P = sm + off.P, *D = sm + off.D;
   bf16* zs = reinterpret_cast<bf16*>(sm + off.z);
   const int conv = 2 * a.nk * DK + a.nv * DV, col0 = cg * DVS;
@@ -219,14 +221,19 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a)
   }
   constexpr int WC = TreeState<DK, DVS>::WC, SL = TreeState<DK, DVS>::SL, VG = TreeState<DK, DVS>::VG, KR = TreeState<DK, DVS>::KR, BV = TreeState<DK, DVS>::BV;
   const int sl = warp % SL;
-  float st[KR][WC];
-  {
-    const float* sp = a.state + (((int64_t)slot * a.nv + h) * DK + sl * KR) * DV + col0 + lane * WC;
+  float st[TILE ? 1 : KR][WC];
+  const float* head = a.state + ((int64_t)slot * a.nv + h) * DK * DV + col0;
+  if (TILE) {
+#pragma unroll 1
+    for (int i = tid; i < DK * DVS / 4; i += kThreads) copy16(P + i * 4, head + (int64_t)(i / (DVS / 4)) * DV + i % (DVS / 4) * 4);
+  } else {
+    const float* sp = head + sl * KR * DV + lane * WC;
 #pragma unroll
     for (int k = 0; k < KR; ++k) {
-      if (WC == 4) *reinterpret_cast<float4*>(st[k]) = *reinterpret_cast<const float4*>(sp + k * DV);
-      else if (WC == 2) *reinterpret_cast<float2*>(st[k]) = *reinterpret_cast<const float2*>(sp + k * DV);
-      else st[k][0] = sp[k * DV];
+      float* x = st[TILE ? 0 : k];
+      if (WC == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(sp + k * DV);
+      else if (WC == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(sp + k * DV);
+      else x[0] = sp[k * DV];
     }
   }
   if (tid < Cp) {
@@ -253,6 +260,60 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a)
   asm volatile("cp.async.wait_all;" ::: "memory");
   __syncthreads();
   // ---- S0^T k and S0^T q (vector v < Cp: row of kn, then of qn)
+  if (TILE) {
+    // 16 groups of columns 4 g + {0..3} and 64 + 4 g + {0..3}, 16 of vectors v0 + 16 n
+    const int c4 = tid % 16 * 4, v0 = tid / 16;
+    float acc[8][8];
+#pragma unroll
+    for (int n = 0; n < 8; ++n)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) acc[n][c] = 0.f;
+    const float* vec[8];
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const int v = min(v0 + 16 * n, 2 * Cp - 1);
+      vec[n] = v < Cp ? kn + v * LK : qn + (v - Cp) * LK;
+    }
+#pragma unroll 1
+    for (int k = 0; k < DK; k += 4) {
+      float4 s[4][2];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        s[e][0] = *reinterpret_cast<const float4*>(P + (k + e) * DVS + c4);
+        s[e][1] = *reinterpret_cast<const float4*>(P + (k + e) * DVS + c4 + DVS / 2);
+      }
+#pragma unroll
+      for (int n = 0; n < 8; ++n) {
+        const float4 x = *reinterpret_cast<const float4*>(vec[n] + k);
+        const float f[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            acc[n][4 * u] = fmaf(f[e], s[e][u].x, acc[n][4 * u]);
+            acc[n][4 * u + 1] = fmaf(f[e], s[e][u].y, acc[n][4 * u + 1]);
+            acc[n][4 * u + 2] = fmaf(f[e], s[e][u].z, acc[n][4 * u + 2]);
+            acc[n][4 * u + 3] = fmaf(f[e], s[e][u].w, acc[n][4 * u + 3]);
+          }
+      }
+    }
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      const int v = v0 + 16 * n, j = v < Cp ? v : v - Cp;
+      if (v >= 2 * Cp) continue;
+      const float f = dec_s[j], b = beta_s[j];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        float4* x = reinterpret_cast<float4*>((v < Cp ? d : o) + j * DVS + c4 + u * (DVS / 2));
+        float4 y = make_float4(f * acc[n][4 * u], f * acc[n][4 * u + 1], f * acc[n][4 * u + 2], f * acc[n][4 * u + 3]);
+        if (v < Cp) {
+          const float4 w = *x;
+          y = make_float4(b * (w.x - y.x), b * (w.y - y.y), b * (w.z - y.z), b * (w.w - y.w));
+        }
+        *x = y;
+      }
+    }
+  } else {
 #pragma unroll 1
   for (int b0 = 0; b0 < 2 * Cp; b0 += BV) {
     const int here = min(BV, 2 * Cp - b0);
@@ -270,10 +331,10 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a)
           const float4 f = *reinterpret_cast<const float4*>(x + n * LK + k);
 #pragma unroll
           for (int c = 0; c < WC; ++c) {
-            acc[n][c] = fmaf(f.x, st[k][c], acc[n][c]);
-            acc[n][c] = fmaf(f.y, st[k + 1][c], acc[n][c]);
-            acc[n][c] = fmaf(f.z, st[k + 2][c], acc[n][c]);
-            acc[n][c] = fmaf(f.w, st[k + 3][c], acc[n][c]);
+            acc[n][c] = fmaf(f.x, st[TILE ? 0 : k][c], acc[n][c]);
+            acc[n][c] = fmaf(f.y, st[TILE ? 0 : k + 1][c], acc[n][c]);
+            acc[n][c] = fmaf(f.z, st[TILE ? 0 : k + 2][c], acc[n][c]);
+            acc[n][c] = fmaf(f.w, st[TILE ? 0 : k + 3][c], acc[n][c]);
           }
         }
       }
@@ -303,6 +364,7 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a)
       } else *x = make_float4(f * s.x, f * s.y, f * s.z, f * s.w);
     }
     if (b0 + BV < 2 * Cp) __syncthreads();
+  }
   }
   sync_all<NS>();                                            // the partial products' place is free, in every CTA of the cluster
   // ---- Gram matrices: A_ji = -beta_j e^{c_j - c_i} k_j.k_i above j, B_ji = e^{c_j - c_i} q_j.k_i above j and at j; 0 elsewhere.  Units of
@@ -477,11 +539,13 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a)
   }
 }
 
-template <int DK, int DV, int DVS>
+template <int DK, int DV, int DVS, bool TILE = false>
 int launch_gdn_tree(const GdnTreeArgs& a, int R, cudaStream_t st) {
-  auto kern = gdn_tree_kernel<DK, DV, DVS>;
-  const size_t smem = TreeSmem<DK, DVS>(a.Cp).total * sizeof(float);
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+  auto kern = gdn_tree_kernel<DK, DV, DVS, TILE>;
+  const size_t smem = TreeSmem<DK, DVS, TILE>(a.Cp).total * sizeof(float);
+  static SmemLimit limit;
+  std::lock_guard<std::mutex> lock(limit.held);
+  cudaError_t e = limit.set(kern, smem);
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(DV / DVS, (unsigned)a.nv, (unsigned)R);
@@ -521,6 +585,7 @@ CB_EXPORT int cb_gdn_tree(const void* proj, int64_t ldp, const void* conv_w, con
   // Up to eight nodes the exchange costs more than it saves: 4 nodes, 32 heads 11.8 / 12.8 / 13.3.
   const int64_t room = 148 / (R * nv);
   const int ns = C <= 8 || room < 2 ? 1 : (room < 4 ? 2 : 4);
+  if (dk == 128 && ns == 1 && C > 48) return launch_gdn_tree<128, 128, 128, true>(a, (int)R, st);
   if (dk == 128) return ns == 1 ? launch_gdn_tree<128, 128, 128>(a, (int)R, st) : ns == 2 ? launch_gdn_tree<128, 128, 64>(a, (int)R, st) : launch_gdn_tree<128, 128, 32>(a, (int)R, st);
   return launch_gdn_tree<64, 64, 32>(a, (int)R, st);              // two CTAs a head
 }

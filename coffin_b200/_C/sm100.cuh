@@ -209,6 +209,23 @@ __device__ __forceinline__ void umma_commit_pair(uint64_t* bar, uint16_t cta_mas
 
 }  // namespace sm100
 
+// ---- host: the dynamic shared memory a kernel may use, set again only where a launch needs another size than the last one on its device
+// (the call costs a sixth of a launch, and a limit above what a launch uses makes that launch slower).  Held from `set` to the launch.
+#include <mutex>
+struct SmemLimit {
+  size_t last[64] = {};
+  std::mutex held;
+  template <typename Kern>
+  cudaError_t set(Kern kern, size_t bytes) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess || (dev < 64 && last[dev] == bytes)) return e;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (dev < 64) last[dev] = e == cudaSuccess ? bytes : 0;
+    return e;
+  }
+};
+
 // ---- host: TMA descriptor encoding through the driver entry point (no link-time libcuda) -----
 #include <cuda.h>
 typedef CUresult (*cb_encode_tiled_fn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

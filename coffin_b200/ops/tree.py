@@ -38,6 +38,7 @@ def _bad(what: str) -> None:
 
 
 _fns: dict[str, object] = {}
+_PLAIN = (int, float)
 # the current stream's handle without a Stream object around it (3 us less a call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
@@ -50,7 +51,7 @@ def call(name: str, *args) -> None:
         fn = _fns[name] = _lib.lib()["cb_" + name]
         fn.restype = ctypes.c_int
         fn.argtypes = [ctypes.c_float if isinstance(a, float) else ctypes.c_int64 if isinstance(a, int) else ctypes.c_void_p for a in args] + [ctypes.c_void_p]
-    rc = fn(*[a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args], _raw_stream(torch.cuda.current_device()))
+    rc = fn(*[a if a is None or a.__class__ in _PLAIN else a.data_ptr() for a in args], _raw_stream(torch.cuda.current_device()))
     if rc:
         raise _lib.KernelError(f"cb_{name} failed: {_lib.ERRORS.get(rc, 'CUDA error')} ({rc})")
 
@@ -199,7 +200,7 @@ def verify_tree(logits, tokens, anc, temperature, u) -> tuple[torch.Tensor, torc
     steps, nxt = torch.empty(R, dtype=torch.int32, device=dev), torch.empty(R, dtype=torch.int64, device=dev)
     if R:
         call("verify_tree", logits, logits.stride(0), logits.stride(1), tokens, anc, temperature, u, path, steps, nxt, torch.empty(_scratch_bytes(R, C, V), dtype=torch.uint8, device=dev), R, C, V)
-        K._count(3)
+        K._count(2)
     return path, steps, nxt
 
 
@@ -229,7 +230,7 @@ def verify_drafts(logits, tokens, lengths, draft_probs, temperature, u, u_draw) 
     if R:
         call("verify_drafts", logits, logits.stride(0), logits.stride(1), tokens, lengths, draft_probs, draft_probs.stride(0) if C > 1 else 0,
              draft_probs.stride(1) if C > 1 else 0, temperature, u, u_draw, steps, nxt, torch.empty(_scratch_bytes(R, C, V), dtype=torch.uint8, device=dev), R, C, V)
-        K._count(3)
+        K._count(2)
     return steps, nxt
 
 
