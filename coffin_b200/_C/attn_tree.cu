@@ -142,8 +142,8 @@ __device__ __forceinline__ uint2 codes_to_bf16(uint32_t w) {
 
 // Stages of the rings, and shared memory: rings of K and V, two tiles of P, int8: two pages of codes.  bf16 pages share one ring of
 // twice as many tiles, in the order of their use: the scores of a page are multiplied while the page before is still in the softmax, so
-// K of a page is requested before V of the page before it.  (With a ring each, V tiles wait for their turn where tiles that are needed
-// earlier could be on their way: 2 x 64 nodes behind 65536 tokens XX -> YY us.)
+// K of a page is requested before V of the page before it.  (With a ring each,
+// a V tile waits for its turn in a place that a K tile could use.)
 template <int HD, bool Q8> struct TreeRing {
   static constexpr int stages = HD == 256 ? (Q8 ? 2 : 3) : HD == 128 ? 4 : 6;
   static constexpr size_t bytes = (size_t)2 * stages * kPage * HD * 2 + 2 * kRows * kPage * 2 + (Q8 ? (size_t)2 * 2 * kPage * HD : 0);

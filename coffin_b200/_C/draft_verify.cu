@@ -168,11 +168,11 @@ __global__ void __launch_bounds__(kNT) row_stats_kernel(const VerifyArgs a) {
     }
     if (T > 0.f) {
       const float floor = fmaxf(mx - 690.f * T, -3.4e38f);
-      if (fabsf(mx) < INFINITY && 690.f * T >= fabsf(mx) * 0x1p-10f) {
+      if (fabsf(mx) < INFINITY && 690.f * T >= fabsf(mx) * 0x1p-10f && T < 1e30f) {
         const double top = (double)mx;
 #pragma unroll
         for (int i = 0; i < kE; ++i) add_weight(sum, x[i], floor, top, s256, roots);
-      } else {                                              // infinite, or so cold that the floor would be rounded onto the maximum
+      } else {                                              // infinite, so cold that the floor would be rounded onto the maximum, or so hot that it has weight
 #pragma unroll 1
         for (int i = 0; i < kE; ++i)
           if (place(c, i) < e) sum += weight(row[place(c, i)], mx, s256);

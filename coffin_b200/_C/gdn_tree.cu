@@ -239,7 +239,8 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a)
   if (tid < Cp) {
     const float x = xa + dtb;
     anc_s[tid] = on;
-    g_s[tid] = on ? fmaxf(-expf(rate) * (x > 20.f ? x : log1pf(expf(x))), -1e4f) : 0.f;      // exp of less is 0 all the same
+    const float g = -expf(rate) * (x > 20.f ? x : log1pf(expf(x)));
+    g_s[tid] = !on ? 0.f : g < -1e4f ? -1e4f : g;             // exp of less is 0 all the same
     beta_s[tid] = 1.f / (1.f + expf(-xb));
   }
   __syncthreads();
@@ -570,7 +571,7 @@ CB_EXPORT int cb_gdn_tree(const void* proj, int64_t ldp, const void* conv_w, con
                           void* record, void* raw, void* rows, int64_t nslots, int64_t R, int64_t C, int64_t nk, int64_t nv, int64_t dk, int64_t dv, float eps,
                           int64_t gate_sigmoid, void* stream) {
   if (!proj || !conv_w || !A_log || !dt_bias || !norm_w || !ring || !state || !slots || !positions || !anc || !out || !record || !raw || !rows) return CB_ERR_ARG;
-  if (R < 1 || R > 65535 || C < 1 || C > kMaxNodes || nk < 1 || nv % nk || nv > 65535 || ldp % 8 || ldo % 4 || ((uintptr_t)out & 7) || ((uintptr_t)norm_w & 15) ||
+  if (R < 1 || R > 65535 || C < 1 || C > kMaxNodes || nk < 1 || nv < 1 || nv % nk || nv > 65535 || ldp % 8 || ldo % 4 || ((uintptr_t)out & 7) || ((uintptr_t)norm_w & 15) ||
       (((uintptr_t)proj | (uintptr_t)ring | (uintptr_t)state | (uintptr_t)raw | (uintptr_t)rows | (uintptr_t)conv_w) & 15)) return CB_ERR_SHAPE;
   GdnTreeArgs a{(const bf16*)proj, ldp, (const float*)conv_w, (const float*)A_log, (const float*)dt_bias, (const float*)norm_w, (const bf16*)ring,
                 (const float*)state, (const int*)slots, (const int*)positions, (const int64_t*)anc, (bf16*)out, ldo, (float*)record, (bf16*)raw, (float*)rows,

@@ -258,6 +258,14 @@ def test_delta_net_of_trees(nk, nv, d, C, positions, kind):
     assert torch.equal(keep[0], a.state) and torch.equal(keep[1], a.ring), "state and ring are read only"
 
 
+@pytest.mark.parametrize("R,C,nk,nv,kind", [(3, 64, 16, 32, "tree"), (5, 49, 4, 16, "tree"), (1, 57, 8, 96, "star"), (2, 63, 38, 38, "chain"),      # a CTA a head
+                                            (2, 33, 8, 24, "tree"), (1, 64, 19, 38, "chain")])                                               # two CTAs a head
+def test_delta_net_of_trees_of_many_heads(R, C, nk, nv, kind):
+    a = Gdn(R, C, nk, nv, 128, list(range(3, 3 + R)), kind, seed=C + nv)
+    a.run()
+    a.check()
+
+
 def test_delta_net_with_sigmoid_gates_wide_rows_and_unused_places():
     a = Gdn(3, 9, 2, 4, 64, [4, 9, 40], parents=[[-1, 0, 1, None, 0, 4, None, 5, None], None, [-1] + list(range(8))], seed=6, pad=24)
     a.run(gate_sigmoid=True)
@@ -288,6 +296,22 @@ def test_delta_net_keeps_what_is_sick_on_its_path():
             assert torch.equal(a.out[j], healthy[0][j]) and torch.equal(a.record[0, j], healthy[1][0, j]), f"node {j}"
         else:
             assert not torch.isfinite(a.out[j].float()).any()
+
+
+@pytest.mark.parametrize("C, kind", [(7, "tree"), (64, "tree")])
+def test_delta_net_keeps_a_sick_gate_on_its_path(C, kind):
+    """A decay that is no number is not taken for some decay: its node and the nodes behind it are none either, the others are what they were."""
+    nv, d = 96, 128
+    a = Gdn(1, C, 2, nv, d, [12], kind, seed=15)
+    a.run()
+    healthy = a.out.clone()
+    a.proj[2, 2 * 2 * d + 2 * nv * d + nv:2 * 2 * d + 2 * nv * d + 2 * nv] = float("nan")
+    a.run()
+    for j in range(C):
+        if 2 in P.path_of(a.parents[0], j):
+            assert not torch.isfinite(a.out[j].float()).any()
+        else:
+            assert torch.equal(a.out[j], healthy[j]), f"node {j}"
 
 
 def test_delta_net_with_decays_of_every_strength():
@@ -391,6 +415,24 @@ def test_verification_at_every_temperature(T):
     for r in range(R):
         want, near = P.choose(P.probs(logits[r, 0], float(temps[r])), float(u[r, 0]))
         assert near > 1e-11 and got[r] == want, r
+
+
+@pytest.mark.parametrize("T", [3e31, 2e36, 3e38])
+def test_masked_tokens_weigh_nothing_at_the_highest_temperatures(T):
+    """At these all weights are 1 or 0 (exp of at most 40 / T); a floor of the type's lowest value over T would have weight."""
+    from coffin_b200.ops import tree
+    V = 5001
+    logits = torch.randn(4, 1, V, generator=_gen(21), device="cuda")
+    keep = torch.arange(0, V, 7, device="cuda")
+    masked = torch.full_like(logits, float("-inf"))
+    masked[:, :, keep] = logits[:, :, keep]
+    one, u = torch.ones(4, 1, dtype=I64, device="cuda"), torch.tensor([[0.01], [0.37], [0.62], [0.99]], device="cuda")
+    got = tree.verify_tree(masked, one, one, torch.full((4,), T, device="cuda"), u)[2].tolist()
+    n = torch.full((4,), 1, dtype=I32, device="cuda")
+    again = tree.verify_drafts(masked, one, n, None, torch.full((4,), T, device="cuda"), u, u[:, 0].contiguous())[1].tolist()
+    for r in range(4):
+        want, near = P.choose(P.probs(masked[r, 0], T), float(u[r, 0]))
+        assert near > 1e-11 and got[r] == want and again[r] == want, r
 
 
 def test_verification_skips_unused_sequences_and_reads_strided_logits():
