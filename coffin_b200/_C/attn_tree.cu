@@ -38,9 +38,9 @@ struct TreeAttnArgs {
   const int* positions;                   // [R] cached tokens (< 0: unused row)
   const int64_t* anc;                     // [R, C]
   bf16* out; int64_t ldo;                 // [R * C, nh * hd]
-  float* part_o;                          // [ctas + items, used rows, hd] unnormalised sums
+  float* part_o;                          // [workers + items, used rows, hd] unnormalised sums
   float* part_ml;                         // the same rows: (reference maximum, sum)
-  int R, C, nh, nkv, rep, tiles, used, ctas;   // tiles: of 128 rows a (sequence, kv head); used: rows of a slot
+  int R, C, nh, nkv, rep, span, tiles, used, workers;      // tiles: of `span` rows a (sequence, kv head); used: rows of a slot; workers: CTAs or pairs
   float scale_log2;                       // hd^-0.5 * log2(e)
   int* status;
 };
@@ -144,26 +144,27 @@ __device__ __forceinline__ uint2 codes_to_bf16(uint32_t w) {
 // twice as many tiles, in the order of their use: the scores of a page are multiplied while the page before is still in the softmax, so
 // K of a page is requested before V of the page before it.  (With a ring each,
 // a V tile waits for its turn in a place that a K tile could use.)
-template <int HD, bool Q8> struct TreeRing {
-  static constexpr int stages = HD == 256 ? (Q8 ? 2 : 3) : HD == 128 ? 4 : 6;
-  static constexpr size_t bytes = (size_t)2 * stages * kPage * HD * 2 + 2 * kRows * kPage * 2 + (Q8 ? (size_t)2 * 2 * kPage * HD : 0);
+template <int HD, bool Q8, bool PAIR> struct TreeRing {
+  static constexpr int half = PAIR ? 2 : 1, stages = (HD == 256 ? (Q8 ? 2 : 3) : HD == 128 ? 4 : 6) * half;
+  static constexpr size_t bytes = (size_t)2 * stages * kPage * HD * 2 / half + 2 * kRows * kPage * 2 + (Q8 ? (size_t)2 * 2 * kPage * HD / half : 0);
 };
 
 // Places of page n's tiles in the order of the shared ring, `total` pages in all.
 __device__ __forceinline__ int unit_k(int n) { return n == 0 ? 0 : 2 * n - 1; }
 __device__ __forceinline__ int unit_v(int n, int total) { return n + 1 < total ? 2 * n + 2 : 2 * n + 1; }
 
-template <int HD, bool Q8>
+template <int HD, bool Q8, bool PAIR>
 __global__ void __launch_bounds__(Q8 ? 352 + kLoaders : 352, 1)
 tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs a) {
-  constexpr int NC = HD / 64, ST = TreeRing<HD, Q8>::stages;
+  constexpr int HALF = PAIR ? 2 : 1, NC = HD / 64, VC = NC / HALF, ST = TreeRing<HD, Q8, PAIR>::stages, SPAN = kRows * HALF;
   // Scales of an int8 page are read until its accumulator is free.  K of page n is converted after the scores of page n - ST, and those
   // were multiplied after the accumulator of page n - ST - 2 was free.
   constexpr int SR = ST + 2;
-  constexpr int KC = kPage * 128, KV_BYTES = kPage * HD * 2, P_BYTES = kRows * kPage * 2;
+  constexpr int KROWS = kPage / HALF, KC = KROWS * 128, VCB = kPage * 128;     // this CTA's keys of a page; 64 channels of them, of the values
+  constexpr int KV_BYTES = kPage * HD * 2 / HALF, P_BYTES = kRows * kPage * 2;
   constexpr uint32_t TMEM_COLS = 2 * kPage + HD + HD / 2 <= 256 ? 256 : 512;
-  constexpr uint32_t IDESC_S = umma_idesc(kRows, kPage, 1, 1);
-  constexpr uint32_t IDESC_O = umma_idesc(kRows, HD, 1, 1) | (1u << 16);     // B operand MN-major
+  constexpr uint32_t IDESC_S = umma_idesc(SPAN, kPage, 1, 1);
+  constexpr uint32_t IDESC_O = umma_idesc(SPAN, HD, 1, 1) | (1u << 16);     // B operand MN-major
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* Ks = smem_raw;                       // the swizzle wants 1024-byte blocks; there is no room to round up
   unsigned char* Ps = Ks + 2 * ST * KV_BYTES;         // [2][P_BYTES]
@@ -178,6 +179,9 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   __shared__ int abort_s;
   volatile int* abort_flag = &abort_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = PAIR ? cluster_ctarank() : 0;
+  const bool lead = rank == 0;
+  const int worker = blockIdx.x / HALF;
   griddep_launch();
   griddep_wait();
   if (smem_u32(smem_raw) & 1023) {
@@ -189,9 +193,9 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     page_sums(a, 0, &none, &all);
     const int per = a.nkv * a.tiles;
     const int64_t T = all * per;
-    const int G = (int)min((int64_t)a.ctas, T);
-    const bool some = (int)blockIdx.x < G;
-    const int64_t lo = some ? piece_start(blockIdx.x, T, G) : 0, hi = some ? piece_start(blockIdx.x + 1, T, G) : 0;
+    const int G = (int)min((int64_t)a.workers, T);
+    const bool some = worker < G;
+    const int64_t lo = some ? piece_start(worker, T, G) : 0, hi = some ? piece_start(worker + 1, T, G) : 0;
     int64_t start = 0;
     int r = 0;
     if (lo < hi)                                      // the sequence of the first page: 32 sequences at a time
@@ -217,30 +221,43 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const int n = lo < hi ? cached_pages(a, r) : 1, it = (int)((lo - start) / n);
       seg_s = Segments{(int)(hi - lo), r, n, it / a.tiles, it % a.tiles, r * per + it, 0, (int)(lo - start) - it * n};
       abort_s = 0;
-      mbar_init(&q_full, 8);
+      mbar_init(&q_full, 8 * HALF);
       mbar_init(&o_full, 1);
-      mbar_init(&o_free, 8);
-      for (int i = 0; i < 2 * ST; ++i) { mbar_init(&k_full[i], Q8 ? kLoaders / 2 : 1); mbar_init(&k_free[i], 1); }
+      mbar_init(&o_free, 8 * HALF);
+      for (int i = 0; i < 2 * ST; ++i) { mbar_init(&k_full[i], Q8 ? kLoaders / 64 * HALF : lead ? HALF : 1); mbar_init(&k_free[i], 1); }
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4); mbar_init(&p_full[i], 4); mbar_init(&p_free[i], 1);
+        mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4 * HALF); mbar_init(&p_full[i], 4 * HALF); mbar_init(&p_free[i], 1);
       }
       for (int i = 0; Q8 && i < SR; ++i) mbar_init(&sc_full[i], 2 * kPage);
       for (int i = 0; i < 4; ++i) { mbar_init(&m_done[i][0], 1); mbar_init(&m_done[i][1], 1); mbar_init(&pair_bar[i], 64); }
       mbar_fence_init();
     }
   }
-  __syncthreads();
+  if (PAIR) cluster_sync_all();                       // both CTAs' barriers exist before either signals the other
+  else __syncthreads();
   Segments seg = seg_s;
-  if (seg.left <= 0) return;                          // no page for this CTA
+  if (seg.left <= 0) return;                          // no page for this CTA (and its pair)
   if (warp == 1) {
-    tmem_alloc(&tmem_base_s, TMEM_COLS);
-    tmem_relinquish();
+    if (PAIR) { tmem_alloc_pair(&tmem_base_s, TMEM_COLS); tmem_relinquish_pair(); }
+    else { tmem_alloc(&tmem_base_s, TMEM_COLS); tmem_relinquish(); }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = tmem_base_s, tmem_o = tmem_base + 2 * kPage, tmem_q = tmem_o + HD;       // S0 | S1 | O | Q
-  auto give_up = [&](int code) { tree_give_up(a.status, abort_flag, code); };
+  auto give_up = [&](int code) {
+    tree_give_up(a.status, abort_flag, code);
+    if (PAIR) st_cluster_u32(map_to_cta(smem_u32(&abort_s), rank ^ 1), 1);
+  };
+  // what the multiplying threads wait for is signalled in the CTA that has them; what they complete, in both
+  auto signal = [&](uint64_t* bar) {
+    if (PAIR) mbar_arrive_cluster(map_to_cta(smem_u32(bar), 0));
+    else mbar_arrive(bar);
+  };
+  auto commit = [&](uint64_t* bar) {
+    if (PAIR) umma_commit_pair(bar, 3);
+    else umma_commit(bar);
+  };
   // tile, barriers and phase of page n
   const int total = seg.left;
   auto k_at = [&](int n) { return Q8 ? n % ST : unit_k(n) % (2 * ST); };
@@ -262,7 +279,11 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (slot0 < 0) mbar_arrive(full);             // no such page: its scores are masked, its values cleared
         else {
           mbar_expect_tx(full, KV_BYTES);
-          for (int c = 0; c < NC; ++c) tma_load_2d(Ks + (u % (2 * ST)) * KV_BYTES + c * KC, map, full, g.kvh * HD + c * 64, (int)slot0);
+          unsigned char* to = Ks + (u % (2 * ST)) * KV_BYTES;
+          if (map == &tmK)
+            for (int c = 0; c < NC; ++c) tma_load_2d(to + c * KC, map, full, g.kvh * HD + c * 64, (int)slot0 + (int)rank * KROWS);
+          else
+            for (int c = 0; c < VC; ++c) tma_load_2d(to + c * VCB, map, full, g.kvh * HD + ((int)rank * VC + c) * 64, (int)slot0);
         }
         return true;
       };
@@ -276,7 +297,7 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     }
   } else if (warp == 1) {
     // ------------------------------------ S = Q K^T ----------------------------------------------
-    if (lane == 0) {
+    if (lead && lane == 0) {
       int n = 0;
       bool ok = true;
       for (int sg = 0; ok && seg.next(a); ++sg) {
@@ -290,16 +311,27 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           for (int c = 0; c < NC; ++c) {
             const uint64_t kd = umma_desc_sw128(Ks + s * KV_BYTES + c * KC);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) umma_f16_ta(tmem_base + sb * kPage, tmem_q + c * 32 + k * 8, kd + 2 * k, IDESC_S, (c | k) != 0);
+            for (int k = 0; k < 4; ++k) {
+              if (PAIR) umma_f16_ta_pair(tmem_base + sb * kPage, tmem_q + c * 32 + k * 8, kd + 2 * k, IDESC_S, (c | k) != 0);
+              else umma_f16_ta(tmem_base + sb * kPage, tmem_q + c * 32 + k * 8, kd + 2 * k, IDESC_S, (c | k) != 0);
+            }
           }
-          umma_commit(&k_free[s]);
-          umma_commit(&s_full[sb]);
+          commit(&k_free[s]);
+          commit(&s_full[sb]);
         }
       }
     }
   } else if (warp == 10) {
     // ------------------------------------ O += P V -----------------------------------------------
-    if (lane == 0) {
+    if (PAIR && !Q8 && !lead) {
+      // nothing is multiplied from here; the tiles that land here are reported to the CTA that does
+      if (lane == 0)
+#pragma unroll 1
+        for (int u = 0; u < 2 * total; ++u) {
+          if (!tree_wait(&k_full[u % (2 * ST)], (u / (2 * ST)) & 1, abort_flag)) { give_up(104); break; }
+          signal(&k_full[u % (2 * ST)]);
+        }
+    } else if (lead && lane == 0) {
       int n = 0;
       bool ok = true;
       for (int sg = 0; ok && seg.next(a); ++sg) {
@@ -309,13 +341,16 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           if (!tree_wait(&p_full[sb], (n >> 1) & 1, abort_flag) || !tree_wait(&k_full[s], v_ph(n), abort_flag)) { give_up(95); ok = false; break; }
           tc_fence_after();
           const uint64_t pd = umma_desc_sw128(Ps + sb * P_BYTES);
-          const uint64_t vd = umma_desc_mn_sw128(Ks + s * KV_BYTES, KC);
+          const uint64_t vd = umma_desc_mn_sw128(Ks + s * KV_BYTES, VCB);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) umma_f16(tmem_o, pd + 2 * k, vd + (uint64_t)(k * 16 * 128 >> 4), IDESC_O, p != seg.p0 || k != 0);
-          umma_commit(&k_free[s]);
-          umma_commit(&p_free[sb]);
+          for (int k = 0; k < 4; ++k) {
+            if (PAIR) umma_f16_pair(tmem_o, pd + 2 * k, vd + (uint64_t)(k * 16 * 128 >> 4), IDESC_O, p != seg.p0 || k != 0);
+            else umma_f16(tmem_o, pd + 2 * k, vd + (uint64_t)(k * 16 * 128 >> 4), IDESC_O, p != seg.p0 || k != 0);
+          }
+          commit(&k_free[s]);
+          commit(&p_free[sb]);
         }
-        if (ok) umma_commit(&o_full);
+        if (ok) commit(&o_full);
       }
     }
   } else if (Q8 && warp >= 11) {
@@ -323,16 +358,19 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     // Half of the loaders take the keys, half the values, each at its own pace.  16 codes of a row are a piece; a quarter warp takes four
     // pieces of each of two rows, so that its bf16 stores hit all banks once.  (Loops are kept short: with every copy unrolled the code
     // of all roles leaves the instruction cache, and a page takes twice as long.)
-    constexpr int NT = kLoaders / 2, PER = kPage * HD / 16 / NT, G4 = HD / 64, CODES = kPage * HD, STEP = NT / 4 / G4;
+    constexpr int NT = kLoaders / 2, PER = kPage * HD / 16 / NT / HALF, CODES = kPage * HD / HALF;
     const int v = (threadIdx.x - 352) / NT, t = (threadIdx.x - 352) % NT;
-    const int row0 = t / 8 / G4 * 2 + t % 8 / 4, c0 = t / 8 % G4 * 4 + t % 4;          // piece i: row0 + i * STEP, c0
+    const int g4 = PAIR && v ? VC : NC, step = NT / 4 / g4;                             // groups of 64 channels here; rows from piece to piece
+    const int row0 = t / 8 / g4 * 2 + t % 8 / 4, c0 = t / 8 % g4 * 4 + t % 4;          // piece i: row0 + i * step, c0
+    const int skip = PAIR && !v ? (int)rank * KROWS : 0, cskip = PAIR && v ? (int)rank * (HD / 2) : 0;       // this CTA's first row and channel of a page
+    const int chunk = v ? VCB : KC;
     const int8_t* pool = (const int8_t*)(v ? a.vpool : a.kpool);
     const float* pscale = v ? a.vscale : a.kscale;
     const float smul = v ? 1.f : a.scale_log2;
     const int64_t pitch = (int64_t)a.nkv * HD;
     unsigned char* const mine = Cs + v * 2 * CODES + t * 16;                            // two pages of this thread's own pieces
-    unsigned char* const to0 = Ks + v * ST * KV_BYTES + (c0 / 4) * KC + row0 * 128;
-    const int piece = (c0 % 4) * 2, at0 = (piece ^ (row0 & 7)) << 4, at1 = ((piece + 1) ^ (row0 & 7)) << 4;      // STEP is a multiple of 8
+    unsigned char* const to0 = Ks + v * ST * KV_BYTES + (c0 / 4) * chunk + row0 * 128;
+    const int piece = (c0 % 4) * 2, at0 = (piece ^ (row0 & 7)) << 4, at1 = ((piece + 1) ^ (row0 & 7)) << 4;      // step is a multiple of 8
     float s0 = 0.f, s1 = 0.f;                         // scale of row t of the page to convert and of the one after it
     Segments ahead = seg;
     int ap = 0;
@@ -352,11 +390,12 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         for (int i = 0; i < PER; ++i) {
           const uint4 x = *reinterpret_cast<const uint4*>(codes + i * NT * 16);
           const uint2 x0 = codes_to_bf16(x.x), x1 = codes_to_bf16(x.y), x2 = codes_to_bf16(x.z), x3 = codes_to_bf16(x.w);
-          *reinterpret_cast<uint4*>(to + i * STEP * 128 + at0) = make_uint4(x0.x, x0.y, x1.x, x1.y);
-          *reinterpret_cast<uint4*>(to + i * STEP * 128 + at1) = make_uint4(x2.x, x2.y, x3.x, x3.y);
+          *reinterpret_cast<uint4*>(to + i * step * 128 + at0) = make_uint4(x0.x, x0.y, x1.x, x1.y);
+          *reinterpret_cast<uint4*>(to + i * step * 128 + at1) = make_uint4(x2.x, x2.y, x3.x, x3.y);
         }
         fence_async_smem();
-        mbar_arrive(&k_full[v * ST + st]);
+        __syncwarp();
+        if (lane == 0) signal(&k_full[v * ST + st]);
       }
       // codes of page n + 2, into the place that was just read, by the same threads
       s0 = s1;
@@ -368,11 +407,11 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const int64_t slot0 = page_slot(a, ahead.r, ap);
         const int valid = slot0 < 0 ? 0 : min(kPage, cached_keys(a, ahead.r) - ap * kPage);
         const uint32_t to = smem_u32(mine + (n & 1) * CODES);
-        const int8_t* from = pool + (valid ? (slot0 + row0) * pitch + ahead.kvh * HD + c0 * 16 : 0);
+        const int8_t* from = pool + (valid ? (slot0 + skip + row0) * pitch + ahead.kvh * HD + cskip + c0 * 16 : 0);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-          const bool in = row0 + i * STEP < valid;    // else zeros, and the address is not read
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * NT * 16), "l"(in ? from + i * STEP * pitch : pool), "r"(in ? 16 : 0));
+          const bool in = skip + row0 + i * step < valid;    // else zeros, and the address is not read
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * NT * 16), "l"(in ? from + i * step * pitch : pool), "r"(in ? 16 : 0));
         }
         s1 = t < valid ? pscale[(slot0 + t) * a.nkv + ahead.kvh] : 0.f;
         ++ap;
@@ -390,7 +429,7 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     unsigned char* const own = Ps + grp * P_BYTES + q * 4096;
     const int sub = lane >> 3, pc = lane & 7;
     auto load_q = [&](const Segments& g) {            // 32 rows of the segment's Q into tensor memory, every other 64 columns a group
-      const int first = g.tile * kRows + q * 32;
+      const int first = g.tile * SPAN + (int)rank * kRows + q * 32;
       if (first < rows) {
         const bf16* qs = a.q + ((int64_t)g.r * a.C * a.nh + g.kvh * a.rep) * HD;
 #pragma unroll 1
@@ -414,7 +453,7 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full);
+      if (lane == 0) signal(&q_full);
     };
     int n = 0;
     bool ok = true;
@@ -423,8 +462,9 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     if (more) load_q(ahead);
     for (int sg = 0; ok && more; ++sg) {
       seg = ahead;
-      const bool idle = seg.tile * kRows + q * 32 >= rows;     // no row in this quadrant: its lanes only keep the barriers going
-      const int keys = cached_keys(a, seg.r), row = seg.tile * kRows + r;
+      const int row_a = seg.tile * SPAN + (int)rank * kRows;     // this CTA's first row
+      const bool idle = row_a + q * 32 >= rows;                // no row in this quadrant: its lanes only keep the barriers going
+      const int keys = cached_keys(a, seg.r), row = row_a + r;
       float m = -INFINITY, l = 0.f;
       for (int p = seg.p0; p < seg.p1; ++p, ++n) {
         const int sb = n & 1, s = n % SR;
@@ -526,16 +566,16 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[sb]);      // the accumulator may take S of page n + 2
+        if (lane == 0) signal(&s_free[sb]);      // the accumulator may take S of page n + 2
         if (!Q8 && valid < kPage) {                   // 0 times what lies behind the cache is not always 0: clear it
           if (!tree_wait(&k_full[v_at(n)], v_ph(n), abort_flag)) { if (lane == 0) give_up(101); ok = false; break; }
           const int per = (kPage - valid) * 8;        // 16-byte pieces of a chunk
-          for (int i = q * 32 + lane; i < NC * per; i += 128)
-            *reinterpret_cast<uint4*>(Ks + v_at(n) * KV_BYTES + (i / per) * KC + valid * 128 + (i % per) * 16) = make_uint4(0, 0, 0, 0);
+          for (int i = q * 32 + lane; i < VC * per; i += 128)
+            *reinterpret_cast<uint4*>(Ks + v_at(n) * KV_BYTES + (i / per) * VCB + valid * 128 + (i % per) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_async_smem();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[sb]);
+        if (lane == 0) signal(&p_full[sb]);
       }
       if (!ok) break;
       if (!tree_wait(&o_full, sg & 1, abort_flag) || !tree_wait(&m_done[q][(n - 1) & 1], ((n - 1) >> 1) & 1, abort_flag)) { if (lane == 0) give_up(102); break; }
@@ -552,10 +592,10 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       mbar_arrive(&pair_bar[q]);
       if (!tree_wait(&pair_bar[q], 1, abort_flag)) { if (lane == 0) give_up(103); break; }
       if (!idle) {
-        const int64_t at = ((int64_t)blockIdx.x + seg.item) * a.used + q * 32;         // the warp's first row
+        const int64_t at = ((int64_t)worker + seg.item) * a.used + (int)rank * kRows + q * 32;         // the warp's first row
         if (grp == 0 && row < rows) *reinterpret_cast<float2*>(a.part_ml + (at + lane) * 2) = make_float2(was, l + reinterpret_cast<const float*>(own)[lane]);
         __syncwarp();
-        const int here = min(32, rows - seg.tile * kRows - q * 32);
+        const int here = min(32, rows - row_a - q * 32);
 #pragma unroll 1
         for (int c0 = grp * (HD / 2); c0 < (grp + 1) * (HD / 2); c0 += 32) {
           uint32_t o[32];
@@ -574,7 +614,7 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&o_free);
+      if (lane == 0) signal(&o_free);
     }
   }
   // ------------------------------------ teardown --------------------------------------------------
@@ -584,9 +624,11 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     const long long t0 = clock64();
     while (clock64() - t0 < 4000000ll) __nanosleep(1000);
   }
+  if (PAIR) cluster_sync_all();                       // the products read and write both CTAs' memory, and both signal each other
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, TMEM_COLS);
+    if (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+    else tmem_dealloc(tmem_base, TMEM_COLS);
   }
 }
 
@@ -647,15 +689,15 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
   // the cache's partials: maxima and sums, one a lane
   int64_t before, all;
   page_sums(a, r, &before, &all);
-  const int n = cached_pages(a, r), per = a.nkv * a.tiles, lrow = j * a.rep + h % a.rep, it = kvh * a.tiles + lrow / kRows, item = r * per + it;
+  const int n = cached_pages(a, r), per = a.nkv * a.tiles, lrow = j * a.rep + h % a.rep, it = kvh * a.tiles + lrow / a.span, item = r * per + it;
   int b0 = 0, parts = 0;
   if (n > 0) {
     const int64_t T = all * per, g0 = before * per + (int64_t)it * n;
-    const int G = (int)min((int64_t)a.ctas, T);
+    const int G = (int)min((int64_t)a.workers, T);
     b0 = piece_of(g0, T, G);
     parts = piece_of(g0 + n - 1, T, G) - b0 + 1;
   }
-  const int64_t at0 = (int64_t)(b0 + item) * a.used + lrow % kRows;
+  const int64_t at0 = (int64_t)(b0 + item) * a.used + lrow % a.span;
   float m = -INFINITY, l = 0.f;
 #pragma unroll 1
   for (int b = lane; b < parts; b += 32) m = fmaxf(m, a.part_ml[(at0 + (int64_t)b * a.used) * 2]);
@@ -754,44 +796,71 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
   }
 }
 
-template <int HD, bool Q8>
-int launch_tree(const TreeAttnArgs& a, int64_t slots, cudaStream_t st) {
+template <int HD, bool Q8, bool PAIR>
+int launch_cache(const TreeAttnArgs& a, int64_t slots, cudaStream_t st) {
   CUtensorMap tmK = {}, tmV = {};
   if (!Q8) {
-    int rc = cb_make_tmap_2d(&tmK, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.kpool, (uint64_t)slots, (uint64_t)a.nkv * HD, (uint64_t)a.nkv * HD, kPage, 64);
+    int rc = cb_make_tmap_2d(&tmK, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.kpool, (uint64_t)slots, (uint64_t)a.nkv * HD, (uint64_t)a.nkv * HD, PAIR ? kPage / 2 : kPage, 64);
     if (!rc) rc = cb_make_tmap_2d(&tmV, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.vpool, (uint64_t)slots, (uint64_t)a.nkv * HD, (uint64_t)a.nkv * HD, kPage, 64);
     if (rc) return rc;
   }
-  const size_t smem = TreeRing<HD, Q8>::bytes;
-  auto kern = tree_cache_kernel<HD, Q8>;
+  const size_t smem = TreeRing<HD, Q8, PAIR>::bytes;
+  auto kern = tree_cache_kernel<HD, Q8, PAIR>;
   static SmemLimit limit;
-  cudaError_t e;
-  {
-    std::lock_guard<std::mutex> lock(limit.held);
-    e = limit.set(kern, smem);
-    if (e == cudaSuccess) e = cb_launch(kern, dim3((unsigned)a.ctas), dim3(Q8 ? 352 + kLoaders : 352), smem, st, tmK, tmV, a);
-  }
+  std::lock_guard<std::mutex> lock(limit.held);
+  cudaError_t e = limit.set(kern, smem);
   if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(PAIR ? 2 * a.workers : a.workers));
+  cfg.blockDim = dim3(Q8 ? 352 + kLoaders : 352);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (g_cb_use_pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (PAIR) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = 2;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = (unsigned)n;
+  if (g_cb_trace_names) cb_trace_name((const void*)kern);
+  return (int)cudaLaunchKernelEx(&cfg, kern, tmK, tmV, a);
+}
+
+template <int HD, bool Q8>
+int launch_tree(const TreeAttnArgs& a, int64_t slots, cudaStream_t st) {
+  int rc;
+  if constexpr (HD >= 128) rc = a.span > kRows ? launch_cache<HD, Q8, true>(a, slots, st) : launch_cache<HD, Q8, false>(a, slots, st);
+  else rc = launch_cache<HD, Q8, false>(a, slots, st);
+  if (rc) return rc;
   const int64_t tasks = (int64_t)a.R * a.C * a.nh;
   return (int)cb_launch(tree_finish_kernel<HD, Q8>, dim3((unsigned)((tasks + 7) / 8)), dim3(256), 0, st, a);
 }
 
 }  // namespace
 
-// part: (ctas + R * nkv * tiles) * used * (hd + 2) floats, tiles = ceil(C * rep / 128), used = min(128, C * rep)
+// part: (ctas * min(rows, 128) + R * nkv * (rows <= 128 ? rows : rows rounded up to 256)) * (hd + 2) floats, rows = C * nh / nkv; `ctas` is even
 CB_EXPORT int cb_attn_tree(const void* q, const void* gate, int64_t ldg, const void* kpool, const void* vpool, int64_t slots,
                            const void* kscale, const void* vscale, const void* tables, int64_t ldbt, int64_t width, const void* positions,
                            const void* anc, void* out, int64_t ldo, void* part, int64_t ctas, int64_t R, int64_t C, int64_t nh, int64_t nkv,
                            int64_t hd, void* status, void* stream) {
   if (!q || !kpool || !vpool || !tables || !positions || !anc || !out || !part || !status) return CB_ERR_ARG;
   if ((kscale == nullptr) != (vscale == nullptr)) return CB_ERR_ARG;
-  if (R < 1 || C < 1 || C > kMaxNodes || nkv < 1 || nh % nkv || ctas < 1 || ctas > 65535 || width < 1 || width > (1 << 24) || R * C * nh > (1ll << 30) || R * width * nkv * ((C * (nh / nkv) + kRows - 1) / kRows) > 0x7fffffff || slots > 0x7fffffff ||
+  if (R < 1 || C < 1 || C > kMaxNodes || nkv < 1 || nh % nkv || ctas < 2 || ctas % 2 || ctas > 65534 || width < 1 || width > (1 << 24) || R * C * nh > (1ll << 30) || R * width * nkv * ((C * (nh / nkv) + kRows - 1) / kRows) > 0x7fffffff || slots > 0x7fffffff ||
       ((uintptr_t)part & 15)) return CB_ERR_SHAPE;
-  const int64_t rows = C * (nh / nkv), tiles = (rows + kRows - 1) / kRows, used = rows < kRows ? rows : kRows;
-  const int64_t places = (ctas + R * nkv * tiles) * used;
+  // More than 128 rows a kv head: pairs of CTAs, each with half of every page.  (64 channels a head cannot be halved.)
+  const int64_t rows = C * (nh / nkv), span = rows > kRows && hd >= 128 ? 2 * kRows : kRows, workers = span > kRows ? ctas / 2 : ctas;
+  const int64_t tiles = (rows + span - 1) / span, used = rows < span ? rows : span;
+  const int64_t places = (workers + R * nkv * tiles) * used;
   TreeAttnArgs a{(const bf16*)q, (const bf16*)gate, ldg, kpool, vpool, (const float*)kscale, (const float*)vscale, (const int*)tables, ldbt,
                  (int)width, (int)(slots / kPage), (const int*)positions, (const int64_t*)anc, (bf16*)out, ldo, (float*)part,
-                 (float*)part + places * hd, (int)R, (int)C, (int)nh, (int)nkv, (int)(nh / nkv), (int)tiles, (int)used, (int)ctas,
+                 (float*)part + places * hd, (int)R, (int)C, (int)nh, (int)nkv, (int)(nh / nkv), (int)span, (int)tiles, (int)used, (int)workers,
                  1.4426950408889634f / sqrtf((float)hd), (int*)status};
   cudaStream_t st = (cudaStream_t)stream;
   if (hd == 256) return kscale ? launch_tree<256, true>(a, slots, st) : launch_tree<256, false>(a, slots, st);
