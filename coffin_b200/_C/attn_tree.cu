@@ -40,13 +40,15 @@ struct TreeAttnArgs {
   bf16* out; int64_t ldo;                 // [R * C, nh * hd]
   float* part_o;                          // [workers + items, used rows, hd] unnormalised sums
   float* part_ml;                         // the same rows: (reference maximum, sum)
+  int* part_pages;                        // what whole_pieces gave
   int R, C, nh, nkv, rep, span, tiles, used, workers;      // tiles: of `span` rows a (sequence, kv head); used: rows of a slot; workers: CTAs or pairs
   float scale_log2;                       // hd^-0.5 * log2(e)
   int* status;
 };
 
 __device__ __forceinline__ int cached_keys(const TreeAttnArgs& a, int r) { return max(0, min(a.positions[r], a.width * kPage)); }
-__device__ __forceinline__ int cached_pages(const TreeAttnArgs& a, int r) { return (cached_keys(a, r) + kPage - 1) / kPage; }
+__device__ __forceinline__ int pages_of(int pos0, int width) { return (max(0, min(pos0, width * kPage)) + kPage - 1) / kPage; }
+__device__ __forceinline__ int cached_pages(const TreeAttnArgs& a, int r) { return pages_of(a.positions[r], a.width); }
 // first slot of a page, or -1 where the table names none of the pool's
 __device__ __forceinline__ int64_t page_slot(const TreeAttnArgs& a, int r, int page) {
   if (page >= a.width) return -1;
@@ -57,13 +59,14 @@ __device__ __forceinline__ int64_t page_slot(const TreeAttnArgs& a, int r, int p
 // are long: out of line, like everything else here that is not on the path of every page.  See the loaders on the size of the code.)
 __device__ __noinline__ int64_t piece_start(int64_t b, int64_t T, int G) { return b * T / G; }
 __device__ __noinline__ int piece_of(int64_t g, int64_t T, int G) { return (int)(((g + 1) * G - 1) / T); }
-// pages of one item of every sequence before `r`, and of all sequences (a warp)
-__device__ __forceinline__ void page_sums(const TreeAttnArgs& a, int r, int64_t* before, int64_t* all) {
+// Sums over the sequences before `r` and over all of them, of f(pages of an item) (a warp)
+template <typename F>
+__device__ __forceinline__ void page_sums(const TreeAttnArgs& a, int r, const F& f, int64_t* before, int64_t* all) {
   const int lane = threadIdx.x & 31;
   int64_t b = 0, t = 0;
 #pragma unroll 1
   for (int i = lane; i < a.R; i += 32) {
-    const int n = cached_pages(a, i);
+    const int n = f(cached_pages(a, i));
     t += n;
     if (i < r) b += n;
   }
@@ -74,6 +77,23 @@ __device__ __forceinline__ void page_sums(const TreeAttnArgs& a, int r, int64_t*
   }
   *before = b;
   *all = t;
+}
+// Pages of a piece if no piece is to hold pages of two items: the smallest L for which ceil(n / L) pieces an item are no more than the
+// workers.  0 where it is kSwitch pages or more above an even share: going from one item to the next costs a worker about as long as
+// kSwitch pages (the sums leave tensor memory, the next Q enters it, and the chain of products starts anew).  us of a pass with whole
+// pieces / with even ones: SWITCH_FIGURES.
+constexpr int kSwitch = 5;
+__device__ __noinline__ int whole_pieces(const int* positions, int R, int width, int workers, int T, int per) {
+  const int lane = threadIdx.x & 31, L = (T + workers - 1) / workers + lane;
+  int64_t pieces = 0;
+#pragma unroll 1
+  for (int r0 = 0; r0 < R; r0 += 32) {
+    const int n = r0 + lane < R ? pages_of(positions[r0 + lane], width) : 0;
+#pragma unroll 1
+    for (int i = 0; i < min(32, R - r0); ++i) pieces += (__shfl_sync(0xffffffffu, n, i) + L - 1) / L;
+  }
+  const unsigned fits = __ballot_sync(0xffffffffu, lane < kSwitch && pieces * per <= workers);
+  return fits ? __shfl_sync(0xffffffffu, L, __ffs(fits) - 1) : 0;
 }
 
 // Segments of a CTA's piece, one after the other.
@@ -126,6 +146,28 @@ __device__ __forceinline__ float tree_ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// two at a time, in one instruction
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t x, uint64_t y, uint64_t z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(x), "l"(y), "l"(z));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t x, uint64_t y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(x), "l"(y));
+  return r;
+}
 // Four int8 codes -> four bf16, exact: 128 + (x & 127) is 0x4300 | (x & 127) as bf16, and 128 or (x < 0) 256 is 0x4300 | (x & 128).
 __device__ __forceinline__ uint2 codes_to_bf16(uint32_t w) {
   uint2 v;
@@ -173,7 +215,7 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   __shared__ uint64_t q_full, k_full[2 * ST], k_free[2 * ST], s_full[2], s_free[2], p_full[2], p_free[2], o_full, o_free,
       m_done[4][2], pair_bar[4], sc_full[Q8 ? SR : 1];
   __shared__ float mref[kRows];                       // reference maxima
-  __shared__ float scales[Q8 ? SR : 1][2][kPage];     // scale_log2 * key scales, value scales
+  __shared__ __align__(16) float scales[Q8 ? SR : 1][2][kPage];     // scale_log2 * key scales, value scales
   __shared__ Segments seg_s;
   __shared__ uint32_t tmem_base_s;
   __shared__ int abort_s;
@@ -190,18 +232,21 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   }
   if (warp == 0) {
     int64_t none, all;
-    page_sums(a, 0, &none, &all);
+    page_sums(a, 0, [](int n) { return n; }, &none, &all);
     const int per = a.nkv * a.tiles;
     const int64_t T = all * per;
-    const int G = (int)min((int64_t)a.workers, T);
-    const bool some = worker < G;
-    const int64_t lo = some ? piece_start(worker, T, G) : 0, hi = some ? piece_start(worker + 1, T, G) : 0;
+    const int G = (int)min((int64_t)a.workers, T), L = T > G ? whole_pieces(a.positions, a.R, a.width, a.workers, (int)T, per) : 0;      // (one page each: nothing to cut)
+    if (blockIdx.x == 0 && lane == 0) *a.part_pages = L;
+    // where the worker's piece begins and ends, in pages of the list or (whole pieces) as a number among all items' pieces
+    const bool some = L ? true : worker < G;
+    const int64_t lo = L ? worker : some ? piece_start(worker, T, G) : 0, hi = L ? worker + 1 : some ? piece_start(worker + 1, T, G) : 0;
     int64_t start = 0;
     int r = 0;
     if (lo < hi)                                      // the sequence of the first page: 32 sequences at a time
 #pragma unroll 1
-      for (;; r += 32) {
-        const int64_t n = r + lane < a.R ? (int64_t)cached_pages(a, r + lane) * per : 0;
+      for (; r < a.R; r += 32) {
+        const int np = r + lane < a.R ? cached_pages(a, r + lane) : 0;
+        const int64_t n = (int64_t)(L ? (np + L - 1) / L : np) * per;
         int64_t incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -218,8 +263,12 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         start += __shfl_sync(0xffffffffu, incl, 31);
       }
     if (lane == 0) {
-      const int n = lo < hi ? cached_pages(a, r) : 1, it = (int)((lo - start) / n);
-      seg_s = Segments{(int)(hi - lo), r, n, it / a.tiles, it % a.tiles, r * per + it, 0, (int)(lo - start) - it * n};
+      seg_s.left = 0;
+      if (lo < hi && r < a.R) {                       // (whole pieces: there may be fewer of them than workers)
+        const int n = cached_pages(a, r), k = L ? (n + L - 1) / L : n, it = (int)((lo - start) / k), i = (int)(lo - start) - it * k;
+        const int p = L ? (int)piece_start(i, n, k) : i;
+        seg_s = Segments{L ? (int)piece_start(i + 1, n, k) - p : (int)(hi - lo), r, n, it / a.tiles, it % a.tiles, r * per + it, 0, p};
+      }
       abort_s = 0;
       mbar_init(&q_full, 8 * HALF);
       mbar_init(&o_full, 1);
@@ -372,8 +421,18 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     unsigned char* const to0 = Ks + v * ST * KV_BYTES + (c0 / 4) * chunk + row0 * 128;
     const int piece = (c0 % 4) * 2, at0 = (piece ^ (row0 & 7)) << 4, at1 = ((piece + 1) ^ (row0 & 7)) << 4;      // step is a multiple of 8
     float s0 = 0.f, s1 = 0.f;                         // scale of row t of the page to convert and of the one after it
+    // page to request next: its segment, its entry of the table (fetched a page ahead of its use) and the keys of its sequence
     Segments ahead = seg;
-    int ap = 0;
+    int ap = 0, id = 0, keys = 0;
+    auto to_next = [&](bool first) {
+      if (first || ++ap == ahead.p1) {
+        if (!ahead.next(a)) return;
+        ap = ahead.p0;
+        keys = cached_keys(a, ahead.r);
+      }
+      id = ap < a.width ? a.tables[(int64_t)ahead.r * a.ldbt + ap] : -1;
+    };
+    to_next(true);
 #pragma unroll 1
     for (int n = -2; n < total; ++n) {
       if (n >= 0) {
@@ -400,12 +459,8 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       // codes of page n + 2, into the place that was just read, by the same threads
       s0 = s1;
       if (n + 2 < total) {
-        if (n == -2 || ap == ahead.p1) {
-          ahead.next(a);
-          ap = ahead.p0;
-        }
-        const int64_t slot0 = page_slot(a, ahead.r, ap);
-        const int valid = slot0 < 0 ? 0 : min(kPage, cached_keys(a, ahead.r) - ap * kPage);
+        const int64_t slot0 = (int64_t)id * kPage;
+        const int valid = (unsigned)id < (unsigned)a.pages ? min(kPage, keys - ap * kPage) : 0;
         const uint32_t to = smem_u32(mine + (n & 1) * CODES);
         const int8_t* from = pool + (valid ? (slot0 + skip + row0) * pitch + ahead.kvh * HD + cskip + c0 * 16 : 0);
 #pragma unroll
@@ -413,8 +468,8 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           const bool in = skip + row0 + i * step < valid;    // else zeros, and the address is not read
           asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * NT * 16), "l"(in ? from + i * step * pitch : pool), "r"(in ? 16 : 0));
         }
-        s1 = t < valid ? pscale[(slot0 + t) * a.nkv + ahead.kvh] : 0.f;
-        ++ap;
+        s1 = t < valid ? pscale[(slot0 + t) * a.nkv + ahead.kvh] : 1.f;
+        to_next(false);
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     }
@@ -473,21 +528,19 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!tree_wait(&s_full[sb], (n >> 1) & 1, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
         if (Q8 && !tree_wait(&sc_full[Q8 ? s : 0], (n / SR) & 1, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
         tc_fence_after();
-        // scores of columns [32 h, 32 h + 32): scaled, int8; raw, bf16.  They are read twice, for the maximum and for the weights, which
-        // leaves half the registers and half the code of holding them.
+        // raw scores of columns [32 h, 32 h + 32).  They are read twice, for the maximum and for the weights, which leaves half the registers
+        // and half the code of holding them.
         auto scores = [&](int h, uint32_t* sv) {
           tmem_ld32(tmem_base + lane_base + sb * kPage + h * 32, sv);
           tmem_ld_wait();
-          if (Q8) {
-#pragma unroll
-            for (int c = 0; c < 32; ++c) sv[c] = __float_as_uint(__uint_as_float(sv[c]) * scales[Q8 ? s : 0][0][h * 32 + c]);
-          }
-          if (valid < kPage) {
+          if (valid < kPage) {                        // (scales behind the end are 1)
 #pragma unroll
             for (int c = 0; c < 32; ++c)
               if (h * 32 + c >= valid) sv[c] = __float_as_uint(-INFINITY);
           }
         };
+        const uint64_t* const ks2 = reinterpret_cast<const uint64_t*>(scales[Q8 ? s : 0][0]);
+        const uint64_t* const vs2 = reinterpret_cast<const uint64_t*>(scales[Q8 ? s : 0][1]);
         float mx = -INFINITY;
         if (!idle) {
           float mx1 = -INFINITY;
@@ -497,8 +550,10 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
             scores(h, sv);
 #pragma unroll
             for (int c = 0; c < 32; c += 2) {
-              mx = fmaxf(mx, __uint_as_float(sv[c]));
-              mx1 = fmaxf(mx1, __uint_as_float(sv[c + 1]));
+              float s0 = __uint_as_float(sv[c]), s1 = __uint_as_float(sv[c + 1]);
+              if (Q8) unpack2(mul2(pack2(s0, s1), ks2[h * 16 + c / 2]), s0, s1);
+              mx = fmaxf(mx, s0);
+              mx1 = fmaxf(mx1, s1);
             }
           }
           mx = fmaxf(mx, mx1);
@@ -541,7 +596,8 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (n >= 2 && !tree_wait(&p_free[sb], ((n - 2) >> 1) & 1, abort_flag)) { if (lane == 0) give_up(100); ok = false; break; }
         if (!idle) {
           unsigned char* prow = Ps + sb * P_BYTES + r * 128;
-          float l0 = 0.f, l1 = 0.f;
+          uint64_t l2 = 0;
+          const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), minus2 = pack2(-ms, -ms);
 #pragma unroll 1
           for (int h = 0; h < 2; ++h) {
             uint32_t sv[32];
@@ -552,16 +608,19 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int k = c * 8 + i * 2;
-                float p0 = __uint_as_float(sv[k]), p1 = __uint_as_float(sv[k + 1]);
-                p0 = tree_ex2(Q8 ? p0 - ms : fmaf(p0, a.scale_log2, -ms));
-                p1 = tree_ex2(Q8 ? p1 - ms : fmaf(p1, a.scale_log2, -ms));
-                l0 += p0; l1 += p1;
-                if (Q8) { p0 *= scales[Q8 ? s : 0][1][h * 32 + k]; p1 *= scales[Q8 ? s : 0][1][h * 32 + k + 1]; }
+                float p0, p1;
+                unpack2(fma2(pack2(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), Q8 ? ks2[h * 16 + k / 2] : scale2, minus2), p0, p1);
+                p0 = tree_ex2(p0);
+                p1 = tree_ex2(p1);
+                l2 = add2(l2, pack2(p0, p1));
+                if (Q8) unpack2(mul2(pack2(p0, p1), vs2[h * 16 + k / 2]), p0, p1);
                 pk[i] = pack_bf162(p0, p1);           // weights rounded to bf16, half a step 2^-8; their sum is not
               }
               *reinterpret_cast<uint4*>(prow + (((h * 4 + c) ^ (r & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
             }
           }
+          float l0, l1;
+          unpack2(l2, l0, l1);
           l += l0 + l1;
         }
         tc_fence_before();
@@ -661,7 +720,7 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
   const int lane = threadIdx.x & 31;
   if (task >= (int64_t)a.R * a.C * a.nh) return;
   const int h = (int)(task % a.nh), j = (int)(task / a.nh % a.C), r = (int)(task / ((int64_t)a.nh * a.C));
-  const int pos0 = a.positions[r];
+  const int pos0 = a.positions[r], L = *a.part_pages;
   uint64_t on = (uint64_t)a.anc[(int64_t)r * a.C + j];
   if (on == 0 || pos0 < 0) return;
   on = (on & (~0ull >> (63 - j))) | 1ull << j;              // a path ends at its node
@@ -688,10 +747,13 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
   }
   // the cache's partials: maxima and sums, one a lane
   int64_t before, all;
-  page_sums(a, r, &before, &all);
+  page_sums(a, r, [L](int n) { return L ? (n + L - 1) / L : n; }, &before, &all);
   const int n = cached_pages(a, r), per = a.nkv * a.tiles, lrow = j * a.rep + h % a.rep, it = kvh * a.tiles + lrow / a.span, item = r * per + it;
   int b0 = 0, parts = 0;
-  if (n > 0) {
+  if (n > 0 && L) {
+    parts = (n + L - 1) / L;
+    b0 = (int)before * per + it * parts;
+  } else if (n > 0) {
     const int64_t T = all * per, g0 = before * per + (int64_t)it * n;
     const int G = (int)min((int64_t)a.workers, T);
     b0 = piece_of(g0, T, G);
@@ -845,7 +907,7 @@ int launch_tree(const TreeAttnArgs& a, int64_t slots, cudaStream_t st) {
 
 }  // namespace
 
-// part: (ctas * min(rows, 128) + R * nkv * (rows <= 128 ? rows : rows rounded up to 256)) * (hd + 2) floats, rows = C * nh / nkv; `ctas` is even
+// part: (ctas * min(rows, 128) + R * nkv * (rows <= 128 ? rows : rows rounded up to 256)) * (hd + 2) + 1 floats, rows = C * nh / nkv; `ctas` is even
 CB_EXPORT int cb_attn_tree(const void* q, const void* gate, int64_t ldg, const void* kpool, const void* vpool, int64_t slots,
                            const void* kscale, const void* vscale, const void* tables, int64_t ldbt, int64_t width, const void* positions,
                            const void* anc, void* out, int64_t ldo, void* part, int64_t ctas, int64_t R, int64_t C, int64_t nh, int64_t nkv,
@@ -860,7 +922,7 @@ CB_EXPORT int cb_attn_tree(const void* q, const void* gate, int64_t ldg, const v
   const int64_t places = (workers + R * nkv * tiles) * used;
   TreeAttnArgs a{(const bf16*)q, (const bf16*)gate, ldg, kpool, vpool, (const float*)kscale, (const float*)vscale, (const int*)tables, ldbt,
                  (int)width, (int)(slots / kPage), (const int*)positions, (const int64_t*)anc, (bf16*)out, ldo, (float*)part,
-                 (float*)part + places * hd, (int)R, (int)C, (int)nh, (int)nkv, (int)(nh / nkv), (int)span, (int)tiles, (int)used, (int)workers,
+                 (float*)part + places * hd, (int*)part + places * (hd + 2), (int)R, (int)C, (int)nh, (int)nkv, (int)(nh / nkv), (int)span, (int)tiles, (int)used, (int)workers,
                  1.4426950408889634f / sqrtf((float)hd), (int*)status};
   cudaStream_t st = (cudaStream_t)stream;
   if (hd == 256) return kscale ? launch_tree<256, true>(a, slots, st) : launch_tree<256, false>(a, slots, st);

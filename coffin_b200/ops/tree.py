@@ -149,7 +149,7 @@ def attn_tree(q, proj, kpool, vpool, block_tables, positions, anc, out, *, nh: i
     rows, status = C * (nh // nkv), K._status.get(i)
     if status is None:
         status = K.status_word(q.device)
-    part = torch.empty((CTAS * min(rows, 128) + R * nkv * (rows if rows <= 128 else -(-rows // 256) * 256)) * (hd + 2), dtype=_F32, device=q.device)
+    part = torch.empty((CTAS * min(rows, 128) + R * nkv * (rows if rows <= 128 else -(-rows // 256) * 256)) * (hd + 2) + 1, dtype=_F32, device=q.device)
     call("attn_tree", i, qp, pp, ldp, kp, vp, slots, ksp, vsp, tp, ldt, pages, posp, anc.data_ptr(), op, ldo, part.data_ptr(), CTAS, R, C, nh, nkv, hd,
          status.data_ptr())
     K._count(2)
