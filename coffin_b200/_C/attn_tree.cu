@@ -710,10 +710,10 @@ template <int EPL, bool Q8> struct RowPiece {
 
 // A warp a (node, head): the node's path, the partial sums of the cache, the gate and the store.  Lanes own hd / 32 channels of a row;
 // lane i also keeps the pool rows of nodes i and i + 32, and the maximum and sum of a partial.  Latency is all there is to it: tables and
-// maxima are fetched by all lanes at once, keys and values of four nodes together, partials four at a time.
+// maxima are fetched by all lanes at once, keys and values of eight nodes together, partials eight at a time.
 template <int HD, bool Q8>
 __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) {
-  constexpr int EPL = HD / 32;
+  constexpr int EPL = HD / 32, kAtOnce = 8;
   griddep_launch();
   griddep_wait();
   const int64_t task = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -764,13 +764,13 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
 #pragma unroll 1
   for (int b = lane; b < parts; b += 32) m = fmaxf(m, a.part_ml[(at0 + (int64_t)b * a.used) * 2]);
   m = warp_max(m);
-  // the path, four nodes at a time: keys and values are requested together
+  // the path, kAtOnce nodes at a time: keys and values are requested together
 #pragma unroll 1
   for (uint64_t rest = path; rest;) {
-    RowPiece<EPL, Q8> kp[4], vp[4];
-    float s[4], kf[4], vf[4];
+    RowPiece<EPL, Q8> kp[kAtOnce], vp[kAtOnce];
+    float s[kAtOnce], kf[kAtOnce], vf[kAtOnce];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kAtOnce; ++k) {
       const int i = rest ? __ffsll((long long)rest) - 1 : -1;
       rest &= rest - 1;
       const int64_t at = i < 32 ? __shfl_sync(0xffffffffu, kr[0], i & 31) : __shfl_sync(0xffffffffu, kr[1], i & 31);
@@ -790,7 +790,7 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
     }
     float mn = m;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kAtOnce; ++k) {
       if (s[k] == 0.f) {                                    // a node (the same for the warp)
         float d = 0.f;
 #pragma unroll
@@ -805,7 +805,7 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
 #pragma unroll
     for (int e = 0; e < EPL; ++e) o[e] *= c;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int k = 0; k < kAtOnce; ++k) {
       const float w = exp2f(s[k] - ms);
       if (lane == 0) l += w;                                // the partials' sums are one a lane
 #pragma unroll
@@ -823,23 +823,24 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
     }
     const int here = min(32, parts - c);
 #pragma unroll 1
-    for (int b = 0; b < here; b += 4) {
-      float x[4][EPL], g[4];
+    for (int b = 0; b < here; b += kAtOnce) {
+      float x[kAtOnce][EPL], g[kAtOnce];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        g[k] = __shfl_sync(0xffffffffu, f, (b + k) & 31);
-        const float* po = a.part_o + (at0 + (int64_t)(c + min(b + k, here - 1)) * a.used) * HD + lane * EPL;
-        if (b + k >= here) g[k] = 0.f;                      // the last one once more, with no weight
-        if (EPL == 8) {
-          *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(po);
-          *reinterpret_cast<float4*>(x[k] + EPL / 2) = *reinterpret_cast<const float4*>(po + 4);
-        } else {
+      for (int k = 0; k < kAtOnce; ++k) {
+        g[k] = b + k < here ? __shfl_sync(0xffffffffu, f, b + k) : 0.f;      // (the same branch for the warp)
+        if (g[k] != 0.f) {
+          const float* po = a.part_o + (at0 + (int64_t)(c + b + k) * a.used) * HD + lane * EPL;
+          if (EPL == 8) {
+            *reinterpret_cast<float4*>(x[k]) = *reinterpret_cast<const float4*>(po);
+            *reinterpret_cast<float4*>(x[k] + EPL / 2) = *reinterpret_cast<const float4*>(po + 4);
+          } else {
 #pragma unroll
-          for (int e = 0; e < EPL; ++e) x[k][e] = po[e];
+            for (int e = 0; e < EPL; ++e) x[k][e] = po[e];
+          }
         }
       }
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
+      for (int k = 0; k < kAtOnce; ++k)
         if (g[k] != 0.f) {
 #pragma unroll
           for (int e = 0; e < EPL; ++e) o[e] = fmaf(g[k], x[k][e], o[e]);
