@@ -11,7 +11,7 @@
 // Cache kernel: an item is (sequence, kv head, 128 rows); the pages of all items form one list that the CTAs, one an SM, cut into even
 // pieces, whatever the lengths.  A CTA walks the segments of its piece; each leaves unnormalised sums, maxima and sums of weights in
 // slot (CTA + item), which is different for any two segments because one of the two grows from segment to segment.
-//   warp 0       TMA: K and V pages into rings (a page of a kv head is a [64 x hd] box of the pool, hd / 64 swizzled [64 x 128 B] blocks)
+//   warp 0       TMA: a page of K or V, hd / 64 swizzled [64 x 128 B] blocks, by one copy (a copy a block: issuing them took longer than a page's products)
 //   warp 1, 10   tcgen05.mma (one thread each): S = Q K^T with Q in tensor memory into one of two accumulators; O += P V
 //   warps 2-9    two groups of 128 threads, a thread a row: one takes the even pages, the other the odd ones, so that the exponentials of a
 //                page run under the maxima of the next.  The reference maximum of a row goes from group to group through shared memory
@@ -317,32 +317,39 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   if (warp == 0) {
     // ------------------------------------ TMA producer ------------------------------------------
     if (!Q8 && lane == 0) {
-      // K of page n, then V of page n - 1
-      Segments vs = seg;
-      int vp = 0, n = 0;
-      bool ok = true, have = false;
-      auto load = [&](const CUtensorMap* map, const Segments& g, int page, int u) {
-        const int64_t slot0 = page_slot(a, g.r, page);
-        if (!tree_wait(&k_free[u % (2 * ST)], (u / (2 * ST) & 1) ^ 1, abort_flag)) { give_up(90); return false; }
-        uint64_t* full = &k_full[u % (2 * ST)];
+      // K of page n, then V of page n - 1.  The table's entry is fetched a page ahead: one thread's latencies add up (500 ns a tile without).
+      int p = 0, id = 0;
+      auto to_next = [&](bool first) {
+        if (first || ++p == seg.p1) {
+          if (!seg.next(a)) return;
+          p = seg.p0;
+        }
+        id = p < a.width ? a.tables[(int64_t)seg.r * a.ldbt + p] : -1;
+      };
+      auto load = [&](const CUtensorMap* map, int u, int slot0, int chunk) {
+        const int at = u % (2 * ST);
+        if (!tree_wait(&k_free[at], (u / (2 * ST) & 1) ^ 1, abort_flag)) { give_up(90); return false; }
+        uint64_t* full = &k_full[at];
         if (slot0 < 0) mbar_arrive(full);             // no such page: its scores are masked, its values cleared
         else {
           mbar_expect_tx(full, KV_BYTES);
-          unsigned char* to = Ks + (u % (2 * ST)) * KV_BYTES;
-          if (map == &tmK)
-            for (int c = 0; c < NC; ++c) tma_load_2d(to + c * KC, map, full, g.kvh * HD + c * 64, (int)slot0 + (int)rank * KROWS);
-          else
-            for (int c = 0; c < VC; ++c) tma_load_2d(to + c * VCB, map, full, g.kvh * HD + ((int)rank * VC + c) * 64, (int)slot0);
+          tma_load_3d(Ks + at * KV_BYTES, map, full, 0, slot0, chunk);
         }
         return true;
       };
-      auto load_v = [&](int i) {
-        if (!have || vp == vs.p1) { have = vs.next(a); vp = vs.p0; }
-        return load(&tmV, vs, vp++, unit_v(i, total));
-      };
-      while (ok && seg.next(a))
-        for (int p = seg.p0; ok && p < seg.p1; ++p, ++n) ok = load(&tmK, seg, p, unit_k(n)) && (n == 0 || load_v(n - 1));
-      if (ok) load_v(n - 1);
+      int v_slot = 0, v_chunk = 0;
+      to_next(true);
+#pragma unroll 1
+      for (int n = 0; n <= total; ++n) {
+        const int slot0 = (unsigned)id < (unsigned)a.pages ? id * kPage : -1, chunk = seg.kvh * NC;
+        if (n < total) {
+          to_next(false);
+          if (!load(&tmK, unit_k(n), slot0 < 0 ? -1 : slot0 + (int)rank * KROWS, chunk)) break;
+        }
+        if (n > 0 && !load(&tmV, unit_v(n - 1, total), v_slot, v_chunk + (int)rank * VC)) break;
+        v_slot = slot0;
+        v_chunk = chunk;
+      }
     }
   } else if (warp == 1) {
     // ------------------------------------ S = Q K^T ----------------------------------------------
@@ -528,15 +535,19 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!tree_wait(&s_full[sb], (n >> 1) & 1, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
         if (Q8 && !tree_wait(&sc_full[Q8 ? s : 0], (n / SR) & 1, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
         tc_fence_after();
-        // raw scores of columns [32 h, 32 h + 32).  They are read twice, for the maximum and for the weights, which leaves half the registers
-        // and half the code of holding them.
-        auto scores = [&](int h, uint32_t* sv) {
-          tmem_ld32(tmem_base + lane_base + sb * kPage + h * 32, sv);
+        // bf16: the scores go to registers whole, and the accumulator is free for the page after next before any exponential (2 x 64 nodes
+        // behind 65536 tokens HOLD_FIGURES).  int8, with half the registers a thread: 32 columns at a time, and twice.
+        uint32_t sv[Q8 ? 32 : kPage];
+        auto scores = [&](int c0) {
+          tmem_ld32(tmem_base + lane_base + sb * kPage + c0, sv);
+          if (!Q8) tmem_ld32(tmem_base + lane_base + sb * kPage + 32, sv + (Q8 ? 0 : 32));
           tmem_ld_wait();
-          if (valid < kPage) {                        // (scales behind the end are 1)
+        };
+        auto mask = [&](int c0) {                     // (int8: scales behind the end are 1)
+          if (valid < kPage) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (h * 32 + c >= valid) sv[c] = __float_as_uint(-INFINITY);
+            for (int c = 0; c < (Q8 ? 32 : kPage); ++c)
+              if (c0 + c >= valid) sv[c] = __float_as_uint(-INFINITY);
           }
         };
         const uint64_t* const ks2 = reinterpret_cast<const uint64_t*>(scales[Q8 ? s : 0][0]);
@@ -545,20 +556,25 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!idle) {
           float mx1 = -INFINITY;
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            uint32_t sv[32];
-            scores(h, sv);
+          for (int c0 = 0; c0 < kPage; c0 += Q8 ? 32 : kPage) {
+            scores(c0);
+            if (!Q8) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) signal(&s_free[sb]);
+            }
+            mask(c0);
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) {
+            for (int c = 0; c < (Q8 ? 32 : kPage); c += 2) {
               float s0 = __uint_as_float(sv[c]), s1 = __uint_as_float(sv[c + 1]);
-              if (Q8) unpack2(mul2(pack2(s0, s1), ks2[h * 16 + c / 2]), s0, s1);
+              if (Q8) unpack2(mul2(pack2(s0, s1), ks2[(c0 + c) / 2]), s0, s1);
               mx = fmaxf(mx, s0);
               mx1 = fmaxf(mx1, s1);
             }
           }
           mx = fmaxf(mx, mx1);
           if (!Q8) mx *= a.scale_log2;
-        }
+        } else if (!Q8 && lane == 0) signal(&s_free[sb]);
         if (p == seg.p0) m = mx;
         else {                                        // the other group has left the reference of the page before
           if (!tree_wait(&m_done[q][sb ^ 1], ((n - 1) >> 1) & 1, abort_flag)) { if (lane == 0) give_up(98); ok = false; break; }
@@ -599,33 +615,37 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           uint64_t l2 = 0;
           const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), minus2 = pack2(-ms, -ms);
 #pragma unroll 1
-          for (int h = 0; h < 2; ++h) {
-            uint32_t sv[32];
-            scores(h, sv);
+          for (int c0 = 0; c0 < kPage; c0 += Q8 ? 32 : kPage) {
+            if (Q8) {
+              scores(c0);
+              mask(c0);
+            }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < (Q8 ? 4 : 8); ++c) {
               uint32_t pk[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const int k = c * 8 + i * 2;
                 float p0, p1;
-                unpack2(fma2(pack2(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), Q8 ? ks2[h * 16 + k / 2] : scale2, minus2), p0, p1);
+                unpack2(fma2(pack2(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), Q8 ? ks2[(c0 + k) / 2] : scale2, minus2), p0, p1);
                 p0 = tree_ex2(p0);
                 p1 = tree_ex2(p1);
                 l2 = add2(l2, pack2(p0, p1));
-                if (Q8) unpack2(mul2(pack2(p0, p1), vs2[h * 16 + k / 2]), p0, p1);
+                if (Q8) unpack2(mul2(pack2(p0, p1), vs2[(c0 + k) / 2]), p0, p1);
                 pk[i] = pack_bf162(p0, p1);           // weights rounded to bf16, half a step 2^-8; their sum is not
               }
-              *reinterpret_cast<uint4*>(prow + (((h * 4 + c) ^ (r & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
+              *reinterpret_cast<uint4*>(prow + (((c0 / 8 + c) ^ (r & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
             }
           }
           float l0, l1;
           unpack2(l2, l0, l1);
           l += l0 + l1;
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) signal(&s_free[sb]);      // the accumulator may take S of page n + 2
+        if (Q8) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) signal(&s_free[sb]);
+        }
         if (!Q8 && valid < kPage) {                   // 0 times what lies behind the cache is not always 0: clear it
           if (!tree_wait(&k_full[v_at(n)], v_ph(n), abort_flag)) { if (lane == 0) give_up(101); ok = false; break; }
           const int per = (kPage - valid) * 8;        // 16-byte pieces of a chunk
@@ -863,8 +883,9 @@ template <int HD, bool Q8, bool PAIR>
 int launch_cache(const TreeAttnArgs& a, int64_t slots, cudaStream_t st) {
   CUtensorMap tmK = {}, tmV = {};
   if (!Q8) {
-    int rc = cb_make_tmap_2d(&tmK, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.kpool, (uint64_t)slots, (uint64_t)a.nkv * HD, (uint64_t)a.nkv * HD, PAIR ? kPage / 2 : kPage, 64);
-    if (!rc) rc = cb_make_tmap_2d(&tmV, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.vpool, (uint64_t)slots, (uint64_t)a.nkv * HD, (uint64_t)a.nkv * HD, kPage, 64);
+    constexpr int NC = HD / 64, half = PAIR ? 2 : 1;
+    int rc = cb_make_tmap_chunks(&tmK, a.kpool, (uint64_t)slots, (uint64_t)a.nkv * NC, kPage / half, NC);
+    if (!rc) rc = cb_make_tmap_chunks(&tmV, a.vpool, (uint64_t)slots, (uint64_t)a.nkv * NC, kPage, NC / half);
     if (rc) return rc;
   }
   const size_t smem = TreeRing<HD, Q8, PAIR>::bytes;
