@@ -187,25 +187,28 @@ __device__ __forceinline__ uint2 codes_to_bf16(uint32_t w) {
 // K of a page is requested before V of the page before it.  (With a ring each,
 // a V tile waits for its turn in a place that a K tile could use.)
 template <int HD, bool Q8, bool PAIR> struct TreeRing {
-  static constexpr int half = PAIR ? 2 : 1, stages = (HD == 256 ? (Q8 ? 2 : 3) : HD == 128 ? 4 : 6) * half;
-  static constexpr size_t bytes = (size_t)2 * stages * kPage * HD * 2 / half + 2 * kRows * kPage * 2 + (Q8 ? (size_t)2 * 2 * kPage * HD / half : 0);
+  static constexpr int half = Q8 && PAIR ? 2 : 1, stages = (HD == 256 ? (Q8 ? 2 : 3) : HD == 128 ? 4 : 6) * half;
+  static constexpr size_t tile = (size_t)kPage * HD * 2 / half, bytes = 2 * stages * tile + 2 * kRows * kPage * 2 + (Q8 ? (size_t)2 * 2 * kPage * HD / half : 0);
 };
 
-// Places of page n's tiles in the order of the shared ring, `total` pages in all.
+// Places of step n's tiles in the order of the shared ring (the one before the last V stays empty).
 __device__ __forceinline__ int unit_k(int n) { return n == 0 ? 0 : 2 * n - 1; }
-__device__ __forceinline__ int unit_v(int n, int total) { return n + 1 < total ? 2 * n + 2 : 2 * n + 1; }
+__device__ __forceinline__ int unit_v(int n) { return 2 * n + 2; }
 
 template <int HD, bool Q8, bool PAIR>
 __global__ void __launch_bounds__(Q8 ? 352 + kLoaders : 352, 1)
 tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs a) {
-  constexpr int HALF = PAIR ? 2 : 1, NC = HD / 64, VC = NC / HALF, ST = TreeRing<HD, Q8, PAIR>::stages, SPAN = kRows * HALF;
+  // bf16 pairs take two pages a step: a page of K each, the two sides of one product of 128 keys (products of 64 keys take 46 cycles per 16
+  // channels, of 128 keys 64 cycles), and half the channels of V of both.  An odd last page has a partner that is none.
+  constexpr bool TWO = PAIR && !Q8;
+  constexpr int HALF = PAIR ? 2 : 1, STEP = TWO ? 2 : 1, NC = HD / 64, VC = NC / HALF, ST = TreeRing<HD, Q8, PAIR>::stages, SPAN = kRows * HALF;
   // Scales of an int8 page are read until its accumulator is free.  K of page n is converted after the scores of page n - ST, and those
   // were multiplied after the accumulator of page n - ST - 2 was free.
   constexpr int SR = ST + 2;
-  constexpr int KROWS = kPage / HALF, KC = KROWS * 128, VCB = kPage * 128;     // this CTA's keys of a page; 64 channels of them, of the values
-  constexpr int KV_BYTES = kPage * HD * 2 / HALF, P_BYTES = kRows * kPage * 2;
+  constexpr int KROWS = Q8 ? kPage / HALF : kPage, KC = KROWS * 128, VCB = kPage * 128;     // a tile's keys; 64 channels of them; of the values
+  constexpr int KV_BYTES = (int)TreeRing<HD, Q8, PAIR>::tile, P_BYTES = kRows * kPage * 2;
   constexpr uint32_t TMEM_COLS = 2 * kPage + HD + HD / 2 <= 256 ? 256 : 512;
-  constexpr uint32_t IDESC_S = umma_idesc(SPAN, kPage, 1, 1);
+  constexpr uint32_t IDESC_S = umma_idesc(SPAN, STEP * kPage, 1, 1);
   constexpr uint32_t IDESC_O = umma_idesc(SPAN, HD, 1, 1) | (1u << 16);     // B operand MN-major
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* Ks = smem_raw;                       // the swizzle wants 1024-byte blocks; there is no room to round up
@@ -307,47 +310,60 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     if (PAIR) umma_commit_pair(bar, 3);
     else umma_commit(bar);
   };
-  // tile, barriers and phase of page n
+  // tile, barriers and phase of page n; pages of a segment with the one that makes it whole steps
   const int total = seg.left;
-  auto k_at = [&](int n) { return Q8 ? n % ST : unit_k(n) % (2 * ST); };
-  auto v_at = [&](int n) { return Q8 ? ST + n % ST : unit_v(n, total) % (2 * ST); };
-  auto k_ph = [&](int n) { return (uint32_t)((Q8 ? n / ST : unit_k(n) / (2 * ST)) & 1); };
-  auto v_ph = [&](int n) { return (uint32_t)((Q8 ? n / ST : unit_v(n, total) / (2 * ST)) & 1); };
+  auto k_at = [&](int n) { return Q8 ? n % ST : unit_k(n / STEP) % (2 * ST); };
+  auto v_at = [&](int n) { return Q8 ? ST + n % ST : unit_v(n / STEP) % (2 * ST); };
+  auto k_ph = [&](int n) { return (uint32_t)((Q8 ? n / ST : unit_k(n / STEP) / (2 * ST)) & 1); };
+  auto v_ph = [&](int n) { return (uint32_t)((Q8 ? n / ST : unit_v(n / STEP) / (2 * ST)) & 1); };
+  auto end_of = [&](const Segments& g) { return TWO ? g.p1 + ((g.p1 - g.p0) & 1) : g.p1; };
 
   if (warp == 0) {
     // ------------------------------------ TMA producer ------------------------------------------
     if (!Q8 && lane == 0) {
-      // K of page n, then V of page n - 1.  The table's entry is fetched a page ahead: one thread's latencies add up (500 ns a tile without).
-      int p = 0, id = 0;
+      // K of step n, then V of step n - 1.  The table's entries are fetched a step ahead: one thread's latencies add up.
+      int p = 0, id[2] = {-1, -1};
       auto to_next = [&](bool first) {
-        if (first || ++p == seg.p1) {
-          if (!seg.next(a)) return;
+        p += STEP;
+        if (first || p >= seg.p1) {
+          if (!seg.next(a)) return false;
           p = seg.p0;
         }
-        id = p < a.width ? a.tables[(int64_t)seg.r * a.ldbt + p] : -1;
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) id[i] = p + i < seg.p1 && p + i < a.width ? a.tables[(int64_t)seg.r * a.ldbt + p + i] : -1;
+        return true;
       };
-      auto load = [&](const CUtensorMap* map, int u, int slot0, int chunk) {
+      // a tile of `parts` copies; slot -1: no such page, its scores are masked, its values cleared
+      auto load = [&](const CUtensorMap* map, int u, int parts, const int* slot, int chunk) {
         const int at = u % (2 * ST);
         if (!tree_wait(&k_free[at], (u / (2 * ST) & 1) ^ 1, abort_flag)) { give_up(90); return false; }
         uint64_t* full = &k_full[at];
-        if (slot0 < 0) mbar_arrive(full);             // no such page: its scores are masked, its values cleared
-        else {
-          mbar_expect_tx(full, KV_BYTES);
-          tma_load_3d(Ks + at * KV_BYTES, map, full, 0, slot0, chunk);
-        }
+        const int bytes = KV_BYTES / parts, some = (slot[0] >= 0) + (parts > 1 && slot[STEP - 1] >= 0);
+        if (some == 0) mbar_arrive(full);
+        else mbar_expect_tx(full, some * bytes);
+#pragma unroll
+        for (int i = 0; i < STEP; ++i)
+          if (i < parts && slot[i] >= 0) tma_load_3d(Ks + at * KV_BYTES + i * bytes, map, full, 0, slot[i], chunk);
         return true;
       };
-      int v_slot = 0, v_chunk = 0;
-      to_next(true);
+      int v_slot[STEP], v_chunk = 0;
+      bool more = to_next(true);
 #pragma unroll 1
-      for (int n = 0; n <= total; ++n) {
-        const int slot0 = (unsigned)id < (unsigned)a.pages ? id * kPage : -1, chunk = seg.kvh * NC;
-        if (n < total) {
-          to_next(false);
-          if (!load(&tmK, unit_k(n), slot0 < 0 ? -1 : slot0 + (int)rank * KROWS, chunk)) break;
+      for (int n = 0;; ++n) {
+        const bool here = more;
+        int slot[STEP];
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) slot[i] = (unsigned)id[i] < (unsigned)a.pages ? id[i] * kPage : -1;
+        const int chunk = seg.kvh * NC;
+        if (here) {
+          more = to_next(false);
+          const int own = lead ? slot[0] : slot[STEP - 1];
+          if (!load(&tmK, unit_k(n), 1, &own, chunk)) break;
         }
-        if (n > 0 && !load(&tmV, unit_v(n - 1, total), v_slot, v_chunk + (int)rank * VC)) break;
-        v_slot = slot0;
+        if (n > 0 && !load(&tmV, unit_v(n - 1), STEP, v_slot, v_chunk + (int)rank * VC)) break;
+        if (!here) break;
+#pragma unroll
+        for (int i = 0; i < STEP; ++i) v_slot[i] = slot[i];
         v_chunk = chunk;
       }
     }
@@ -359,9 +375,10 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       for (int sg = 0; ok && seg.next(a); ++sg) {
         if (!tree_wait(&q_full, sg & 1, abort_flag)) { give_up(92); break; }
         tc_fence_after();
-        for (int p = seg.p0; p < seg.p1; ++p, ++n) {
+        for (int p = seg.p0; p < seg.p1; p += STEP, n += STEP) {
           const int s = k_at(n), sb = n & 1;
-          if (!tree_wait(&k_full[s], k_ph(n), abort_flag) || !tree_wait(&s_free[sb], ((n >> 1) & 1) ^ 1, abort_flag)) { give_up(93); ok = false; break; }
+          if (!tree_wait(&k_full[s], k_ph(n), abort_flag) || !tree_wait(&s_free[sb], ((n >> 1) & 1) ^ 1, abort_flag) ||
+              (TWO && !tree_wait(&s_free[1], ((n >> 1) & 1) ^ 1, abort_flag))) { give_up(93); ok = false; break; }
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < NC; ++c) {
@@ -374,36 +391,41 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           }
           commit(&k_free[s]);
           commit(&s_full[sb]);
+          if (TWO) commit(&s_full[1]);
         }
       }
     }
   } else if (warp == 10) {
     // ------------------------------------ O += P V -----------------------------------------------
-    if (PAIR && !Q8 && !lead) {
+    if (TWO && !lead) {
       // nothing is multiplied from here; the tiles that land here are reported to the CTA that does
-      if (lane == 0)
+      if (lane == 0) {
+        int steps = 0;
+        while (seg.next(a)) steps += (end_of(seg) - seg.p0) / STEP;
 #pragma unroll 1
-        for (int u = 0; u < 2 * total; ++u) {
+        for (int u = 0; u <= 2 * steps; ++u) {
+          if (u == 2 * steps - 1) continue;
           if (!tree_wait(&k_full[u % (2 * ST)], (u / (2 * ST)) & 1, abort_flag)) { give_up(104); break; }
           signal(&k_full[u % (2 * ST)]);
         }
+      }
     } else if (lead && lane == 0) {
       int n = 0;
       bool ok = true;
       for (int sg = 0; ok && seg.next(a); ++sg) {
         if (!tree_wait(&o_free, (sg & 1) ^ 1, abort_flag)) { give_up(94); break; }
-        for (int p = seg.p0; p < seg.p1; ++p, ++n) {
+        for (int p = seg.p0; p < end_of(seg); ++p, ++n) {
           const int s = v_at(n), sb = n & 1;
           if (!tree_wait(&p_full[sb], (n >> 1) & 1, abort_flag) || !tree_wait(&k_full[s], v_ph(n), abort_flag)) { give_up(95); ok = false; break; }
           tc_fence_after();
           const uint64_t pd = umma_desc_sw128(Ps + sb * P_BYTES);
-          const uint64_t vd = umma_desc_mn_sw128(Ks + s * KV_BYTES, VCB);
+          const uint64_t vd = umma_desc_mn_sw128(Ks + s * KV_BYTES + (TWO ? sb * (KV_BYTES / 2) : 0), VCB);
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             if (PAIR) umma_f16_pair(tmem_o, pd + 2 * k, vd + (uint64_t)(k * 16 * 128 >> 4), IDESC_O, p != seg.p0 || k != 0);
             else umma_f16(tmem_o, pd + 2 * k, vd + (uint64_t)(k * 16 * 128 >> 4), IDESC_O, p != seg.p0 || k != 0);
           }
-          commit(&k_free[s]);
+          if (!TWO || sb) commit(&k_free[s]);
           commit(&p_free[sb]);
         }
         if (ok) commit(&o_full);
@@ -528,10 +550,10 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       const bool idle = row_a + q * 32 >= rows;                // no row in this quadrant: its lanes only keep the barriers going
       const int keys = cached_keys(a, seg.r), row = row_a + r;
       float m = -INFINITY, l = 0.f;
-      for (int p = seg.p0; p < seg.p1; ++p, ++n) {
+      for (int p = seg.p0; p < end_of(seg); ++p, ++n) {
         const int sb = n & 1, s = n % SR;
         if (sb != grp) continue;
-        const int valid = page_slot(a, seg.r, p) < 0 ? 0 : min(kPage, keys - p * kPage);
+        const int valid = (TWO && p >= seg.p1) || page_slot(a, seg.r, p) < 0 ? 0 : min(kPage, keys - p * kPage);
         if (!tree_wait(&s_full[sb], (n >> 1) & 1, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
         if (Q8 && !tree_wait(&sc_full[Q8 ? s : 0], (n / SR) & 1, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
         tc_fence_after();
@@ -650,7 +672,7 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           if (!tree_wait(&k_full[v_at(n)], v_ph(n), abort_flag)) { if (lane == 0) give_up(101); ok = false; break; }
           const int per = (kPage - valid) * 8;        // 16-byte pieces of a chunk
           for (int i = q * 32 + lane; i < VC * per; i += 128)
-            *reinterpret_cast<uint4*>(Ks + v_at(n) * KV_BYTES + (i / per) * VCB + valid * 128 + (i % per) * 16) = make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>(Ks + v_at(n) * KV_BYTES + (TWO ? sb * (KV_BYTES / 2) : 0) + (i / per) * VCB + valid * 128 + (i % per) * 16) = make_uint4(0, 0, 0, 0);
         }
         fence_async_smem();
         __syncwarp();
@@ -884,7 +906,7 @@ int launch_cache(const TreeAttnArgs& a, int64_t slots, cudaStream_t st) {
   CUtensorMap tmK = {}, tmV = {};
   if (!Q8) {
     constexpr int NC = HD / 64, half = PAIR ? 2 : 1;
-    int rc = cb_make_tmap_chunks(&tmK, a.kpool, (uint64_t)slots, (uint64_t)a.nkv * NC, kPage / half, NC);
+    int rc = cb_make_tmap_chunks(&tmK, a.kpool, (uint64_t)slots, (uint64_t)a.nkv * NC, kPage, NC);
     if (!rc) rc = cb_make_tmap_chunks(&tmV, a.vpool, (uint64_t)slots, (uint64_t)a.nkv * NC, kPage, NC / half);
     if (rc) return rc;
   }
