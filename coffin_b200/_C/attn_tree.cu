@@ -55,28 +55,25 @@ __device__ __forceinline__ int64_t page_slot(const TreeAttnArgs& a, int r, int p
   const int id = a.tables[(int64_t)r * a.ldbt + page];
   return (unsigned)id < (unsigned)a.pages ? (int64_t)id * kPage : -1;
 }
-// The list of all items' T pages, cut into G even pieces (at most one a page): piece b is [b T / G, (b + 1) T / G).  (64-bit divisions
-// are long: out of line, like everything else here that is not on the path of every page.  See the loaders on the size of the code.)
-__device__ __noinline__ int64_t piece_start(int64_t b, int64_t T, int G) { return b * T / G; }
-__device__ __noinline__ int piece_of(int64_t g, int64_t T, int G) { return (int)(((g + 1) * G - 1) / T); }
+// The list of all items' T < 2^31 pages, cut into G even pieces (at most one a page), the first T % G of them a page longer.
+__device__ __forceinline__ int piece_start(int b, int T, int G) { return b * (T / G) + min(b, T % G); }
+__device__ __forceinline__ int piece_of(int g, int T, int G) {
+  const int q = T / G, rest = T % G, longer = rest * (q + 1);
+  return g < longer ? g / (q + 1) : rest + (g - longer) / q;
+}
 // Sums over the sequences before `r` and over all of them, of f(pages of an item) (a warp)
 template <typename F>
-__device__ __forceinline__ void page_sums(const TreeAttnArgs& a, int r, const F& f, int64_t* before, int64_t* all) {
+__device__ __forceinline__ void page_sums(const TreeAttnArgs& a, int r, const F& f, int* before, int* all) {
   const int lane = threadIdx.x & 31;
-  int64_t b = 0, t = 0;
+  int b = 0, t = 0;
 #pragma unroll 1
   for (int i = lane; i < a.R; i += 32) {
     const int n = f(cached_pages(a, i));
     t += n;
     if (i < r) b += n;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    b += __shfl_xor_sync(0xffffffffu, b, o);
-    t += __shfl_xor_sync(0xffffffffu, t, o);
-  }
-  *before = b;
-  *all = t;
+  *before = __reduce_add_sync(0xffffffffu, b);
+  *all = __reduce_add_sync(0xffffffffu, t);
 }
 // Pages of a piece if no piece is to hold pages of two items: the smallest L for which ceil(n / L) pieces an item are no more than the
 // workers.  0 where it is kSwitch pages or more above an even share: going from one item to the next costs a worker about as long as
@@ -85,14 +82,14 @@ __device__ __forceinline__ void page_sums(const TreeAttnArgs& a, int r, const F&
 constexpr int kSwitch = 5;
 __device__ __noinline__ int whole_pieces(const int* positions, int R, int width, int workers, int T, int per) {
   const int lane = threadIdx.x & 31, L = (T + workers - 1) / workers + lane;
-  int64_t pieces = 0;
+  int pieces = 0;
 #pragma unroll 1
   for (int r0 = 0; r0 < R; r0 += 32) {
     const int n = r0 + lane < R ? pages_of(positions[r0 + lane], width) : 0;
 #pragma unroll 1
     for (int i = 0; i < min(32, R - r0); ++i) pieces += (__shfl_sync(0xffffffffu, n, i) + L - 1) / L;
   }
-  const unsigned fits = __ballot_sync(0xffffffffu, lane < kSwitch && pieces * per <= workers);
+  const unsigned fits = __ballot_sync(0xffffffffu, lane < kSwitch && (int64_t)pieces * per <= workers);
   return fits ? __shfl_sync(0xffffffffu, L, __ffs(fits) - 1) : 0;
 }
 
@@ -234,26 +231,23 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     return;
   }
   if (warp == 0) {
-    int64_t none, all;
+    int none, all;
     page_sums(a, 0, [](int n) { return n; }, &none, &all);
-    const int per = a.nkv * a.tiles;
-    const int64_t T = all * per;
-    const int G = (int)min((int64_t)a.workers, T), L = T > G ? whole_pieces(a.positions, a.R, a.width, a.workers, (int)T, per) : 0;      // (one page each: nothing to cut)
+    const int per = a.nkv * a.tiles, T = all * per, G = min(a.workers, T);
+    const int L = T > G ? whole_pieces(a.positions, a.R, a.width, a.workers, T, per) : 0;      // (one page each: nothing to cut)
     if (blockIdx.x == 0 && lane == 0) *a.part_pages = L;
     // where the worker's piece begins and ends, in pages of the list or (whole pieces) as a number among all items' pieces
     const bool some = L ? true : worker < G;
-    const int64_t lo = L ? worker : some ? piece_start(worker, T, G) : 0, hi = L ? worker + 1 : some ? piece_start(worker + 1, T, G) : 0;
-    int64_t start = 0;
-    int r = 0;
+    const int lo = L ? worker : some ? piece_start(worker, T, G) : 0, hi = L ? worker + 1 : some ? piece_start(worker + 1, T, G) : 0;
+    int start = 0, r = 0;
     if (lo < hi)                                      // the sequence of the first page: 32 sequences at a time
 #pragma unroll 1
       for (; r < a.R; r += 32) {
-        const int np = r + lane < a.R ? cached_pages(a, r + lane) : 0;
-        const int64_t n = (int64_t)(L ? (np + L - 1) / L : np) * per;
-        int64_t incl = n;
+        const int np = r + lane < a.R ? cached_pages(a, r + lane) : 0, n = (L ? (np + L - 1) / L : np) * per;
+        int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-          const int64_t x = __shfl_up_sync(0xffffffffu, incl, o);
+          const int x = __shfl_up_sync(0xffffffffu, incl, o);
           if (lane >= o) incl += x;
         }
         const unsigned hit = __ballot_sync(0xffffffffu, start + incl > lo);
@@ -268,10 +262,16 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
     if (lane == 0) {
       seg_s.left = 0;
       if (lo < hi && r < a.R) {                       // (whole pieces: there may be fewer of them than workers)
-        const int n = cached_pages(a, r), k = L ? (n + L - 1) / L : n, it = (int)((lo - start) / k), i = (int)(lo - start) - it * k;
-        const int p = L ? (int)piece_start(i, n, k) : i;
-        seg_s = Segments{L ? (int)piece_start(i + 1, n, k) - p : (int)(hi - lo), r, n, it / a.tiles, it % a.tiles, r * per + it, 0, p};
+        const int n = cached_pages(a, r), k = L ? (n + L - 1) / L : n, it = (lo - start) / k, i = lo - start - it * k;
+        const int p = L ? piece_start(i, n, k) : i;
+        seg_s = Segments{L ? piece_start(i + 1, n, k) - p : hi - lo, r, n, it / a.tiles, it % a.tiles, r * per + it, 0, p};
       }
+    }
+  } else if (warp == 1) {                             // beside it
+    if (PAIR) { tmem_alloc_pair(&tmem_base_s, TMEM_COLS); tmem_relinquish_pair(); }
+    else { tmem_alloc(&tmem_base_s, TMEM_COLS); tmem_relinquish(); }
+  } else if (warp == 2) {
+    if (lane == 0) {
       abort_s = 0;
       mbar_init(&q_full, 8 * HALF);
       mbar_init(&o_full, 1);
@@ -285,18 +285,19 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
       mbar_fence_init();
     }
   }
+  tc_fence_before();
   if (PAIR) cluster_sync_all();                       // both CTAs' barriers exist before either signals the other
   else __syncthreads();
-  Segments seg = seg_s;
-  if (seg.left <= 0) return;                          // no page for this CTA (and its pair)
-  if (warp == 1) {
-    if (PAIR) { tmem_alloc_pair(&tmem_base_s, TMEM_COLS); tmem_relinquish_pair(); }
-    else { tmem_alloc(&tmem_base_s, TMEM_COLS); tmem_relinquish(); }
-  }
-  tc_fence_before();
-  __syncthreads();
   tc_fence_after();
+  Segments seg = seg_s;
   const uint32_t tmem_base = tmem_base_s, tmem_o = tmem_base + 2 * kPage, tmem_q = tmem_o + HD;       // S0 | S1 | O | Q
+  if (seg.left <= 0) {                                // no page for this CTA (and its pair)
+    if (warp == 1) {
+      if (PAIR) tmem_dealloc_pair(tmem_base, TMEM_COLS);
+      else tmem_dealloc(tmem_base, TMEM_COLS);
+    }
+    return;
+  }
   auto give_up = [&](int code) {
     tree_give_up(a.status, abort_flag, code);
     if (PAIR) st_cluster_u32(map_to_cta(smem_u32(&abort_s), rank ^ 1), 1);
@@ -788,16 +789,15 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
     path |= (uint64_t)__ballot_sync(0xffffffffu, slot0 >= 0) << (32 * u);
   }
   // the cache's partials: maxima and sums, one a lane
-  int64_t before, all;
+  int before, all;
   page_sums(a, r, [L](int n) { return L ? (n + L - 1) / L : n; }, &before, &all);
   const int n = cached_pages(a, r), per = a.nkv * a.tiles, lrow = j * a.rep + h % a.rep, it = kvh * a.tiles + lrow / a.span, item = r * per + it;
   int b0 = 0, parts = 0;
   if (n > 0 && L) {
     parts = (n + L - 1) / L;
-    b0 = (int)before * per + it * parts;
+    b0 = before * per + it * parts;
   } else if (n > 0) {
-    const int64_t T = all * per, g0 = before * per + (int64_t)it * n;
-    const int G = (int)min((int64_t)a.workers, T);
+    const int T = all * per, g0 = before * per + it * n, G = min(a.workers, T);
     b0 = piece_of(g0, T, G);
     parts = piece_of(g0 + n - 1, T, G) - b0 + 1;
   }
