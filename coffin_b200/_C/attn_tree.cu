@@ -11,7 +11,7 @@
 // Cache kernel: an item is (sequence, kv head, 128 rows); the pages of all items form one list that the CTAs, one an SM, cut into even
 // pieces, whatever the lengths.  A CTA walks the segments of its piece; each leaves unnormalised sums, maxima and sums of weights in
 // slot (CTA + item), which is different for any two segments because one of the two grows from segment to segment.
-//   warp 0       TMA: a page of K or V, hd / 64 swizzled [64 x 128 B] blocks, by one copy (a copy a block: issuing them took longer than a page's products)
+//   warp 0       TMA: K and V pages into rings (a page of a kv head is a [64 x hd] box of the pool, hd / 64 swizzled [64 x 128 B] blocks)
 //   warp 1, 10   tcgen05.mma (one thread each): S = Q K^T with Q in tensor memory into one of two accumulators; O += P V
 //   warps 2-9    two groups of 128 threads, a thread a row: one takes the even pages, the other the odd ones, so that the exponentials of a
 //                page run under the maxima of the next.  The reference maximum of a row goes from group to group through shared memory
@@ -78,8 +78,8 @@ __device__ __forceinline__ void page_sums(const TreeAttnArgs& a, int r, const F&
 // Pages of a piece if no piece is to hold pages of two items: the smallest L for which ceil(n / L) pieces an item are no more than the
 // workers.  0 where it is kSwitch pages or more above an even share: going from one item to the next costs a worker about as long as
 // kSwitch pages (the sums leave tensor memory, the next Q enters it, and the chain of products starts anew).  us of a pass with whole
-// pieces / with even ones: SWITCH_FIGURES.
-constexpr int kSwitch = 5;
+// pieces / with even ones: 8 x 16 nodes behind 517 to 16391 tokens 64 / 76, 4 x 23 behind up to 8191 (int8) 52 / 56, 2 x 64 behind 65536 133 / 140.
+constexpr int kSwitch = 8;
 __device__ __noinline__ int whole_pieces(const int* positions, int R, int width, int workers, int T, int per) {
   const int lane = threadIdx.x & 31, L = (T + workers - 1) / workers + lane;
   int pieces = 0;
@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(Q8 ? 352 + kLoaders : 352, 1)
 tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs a) {
   // bf16 pairs take two pages a step: a page of K each, the two sides of one product of 128 keys (products of 64 keys take 46 cycles per 16
   // channels, of 128 keys 64 cycles), and half the channels of V of both.  An odd last page has a partner that is none.
-  constexpr bool TWO = PAIR && !Q8;
+  constexpr bool TWO = PAIR && !Q8, HOLD = TWO;
   constexpr int HALF = PAIR ? 2 : 1, STEP = TWO ? 2 : 1, NC = HD / 64, VC = NC / HALF, ST = TreeRing<HD, Q8, PAIR>::stages, SPAN = kRows * HALF;
   // Scales of an int8 page are read until its accumulator is free.  K of page n is converted after the scores of page n - ST, and those
   // were multiplied after the accumulator of page n - ST - 2 was free.
@@ -344,7 +344,9 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         else mbar_expect_tx(full, some * bytes);
 #pragma unroll
         for (int i = 0; i < STEP; ++i)
-          if (i < parts && slot[i] >= 0) tma_load_3d(Ks + at * KV_BYTES + i * bytes, map, full, 0, slot[i], chunk);
+          if (i < parts && slot[i] >= 0)
+#pragma unroll
+            for (int c = 0; c < (map == &tmK ? NC : VC); ++c) tma_load_2d(Ks + at * KV_BYTES + i * bytes + c * VCB, map, full, (chunk + c) * 64, slot[i]);
         return true;
       };
       int v_slot[STEP], v_chunk = 0;
@@ -558,18 +560,19 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!tree_wait(&s_full[sb], (n >> 1) & 1, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
         if (Q8 && !tree_wait(&sc_full[Q8 ? s : 0], (n / SR) & 1, abort_flag)) { if (lane == 0) give_up(97); ok = false; break; }
         tc_fence_after();
-        // bf16: the scores go to registers whole, and the accumulator is free for the page after next before any exponential (2 x 64 nodes
-        // behind 65536 tokens HOLD_FIGURES).  int8, with half the registers a thread: 32 columns at a time, and twice.
-        uint32_t sv[Q8 ? 32 : kPage];
+        // Two pages a product: the scores go to registers whole, and the accumulators are free for the next product before any exponential
+        // (2 x 64 nodes behind 65536 tokens 131 us, freed behind them 174).  Else 32 columns at a time, and twice, which leaves half the
+        // registers and half the code (8 x 16 nodes behind up to 16391 tokens 64.1 us, whole 65.6).
+        uint32_t sv[HOLD ? kPage : 32];
         auto scores = [&](int c0) {
           tmem_ld32(tmem_base + lane_base + sb * kPage + c0, sv);
-          if (!Q8) tmem_ld32(tmem_base + lane_base + sb * kPage + 32, sv + (Q8 ? 0 : 32));
+          if (HOLD) tmem_ld32(tmem_base + lane_base + sb * kPage + 32, sv + (HOLD ? 32 : 0));
           tmem_ld_wait();
         };
         auto mask = [&](int c0) {                     // (int8: scales behind the end are 1)
           if (valid < kPage) {
 #pragma unroll
-            for (int c = 0; c < (Q8 ? 32 : kPage); ++c)
+            for (int c = 0; c < (HOLD ? kPage : 32); ++c)
               if (c0 + c >= valid) sv[c] = __float_as_uint(-INFINITY);
           }
         };
@@ -579,16 +582,16 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!idle) {
           float mx1 = -INFINITY;
 #pragma unroll 1
-          for (int c0 = 0; c0 < kPage; c0 += Q8 ? 32 : kPage) {
+          for (int c0 = 0; c0 < kPage; c0 += HOLD ? kPage : 32) {
             scores(c0);
-            if (!Q8) {
+            if (HOLD) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) signal(&s_free[sb]);
             }
             mask(c0);
 #pragma unroll
-            for (int c = 0; c < (Q8 ? 32 : kPage); c += 2) {
+            for (int c = 0; c < (HOLD ? kPage : 32); c += 2) {
               float s0 = __uint_as_float(sv[c]), s1 = __uint_as_float(sv[c + 1]);
               if (Q8) unpack2(mul2(pack2(s0, s1), ks2[(c0 + c) / 2]), s0, s1);
               mx = fmaxf(mx, s0);
@@ -597,7 +600,7 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           }
           mx = fmaxf(mx, mx1);
           if (!Q8) mx *= a.scale_log2;
-        } else if (!Q8 && lane == 0) signal(&s_free[sb]);
+        } else if (HOLD && lane == 0) signal(&s_free[sb]);
         if (p == seg.p0) m = mx;
         else {                                        // the other group has left the reference of the page before
           if (!tree_wait(&m_done[q][sb ^ 1], ((n - 1) >> 1) & 1, abort_flag)) { if (lane == 0) give_up(98); ok = false; break; }
@@ -638,13 +641,13 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           uint64_t l2 = 0;
           const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), minus2 = pack2(-ms, -ms);
 #pragma unroll 1
-          for (int c0 = 0; c0 < kPage; c0 += Q8 ? 32 : kPage) {
-            if (Q8) {
+          for (int c0 = 0; c0 < kPage; c0 += HOLD ? kPage : 32) {
+            if (!HOLD) {
               scores(c0);
               mask(c0);
             }
 #pragma unroll
-            for (int c = 0; c < (Q8 ? 4 : 8); ++c) {
+            for (int c = 0; c < (HOLD ? 8 : 4); ++c) {
               uint32_t pk[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -664,7 +667,7 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           unpack2(l2, l0, l1);
           l += l0 + l1;
         }
-        if (Q8) {
+        if (!HOLD) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) signal(&s_free[sb]);
@@ -905,9 +908,8 @@ template <int HD, bool Q8, bool PAIR>
 int launch_cache(const TreeAttnArgs& a, int64_t slots, cudaStream_t st) {
   CUtensorMap tmK = {}, tmV = {};
   if (!Q8) {
-    constexpr int NC = HD / 64, half = PAIR ? 2 : 1;
-    int rc = cb_make_tmap_chunks(&tmK, a.kpool, (uint64_t)slots, (uint64_t)a.nkv * NC, kPage, NC);
-    if (!rc) rc = cb_make_tmap_chunks(&tmV, a.vpool, (uint64_t)slots, (uint64_t)a.nkv * NC, kPage, NC / half);
+    int rc = cb_make_tmap_2d(&tmK, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.kpool, (uint64_t)slots, (uint64_t)a.nkv * HD, (uint64_t)a.nkv * HD, kPage, 64);
+    if (!rc) rc = cb_make_tmap_2d(&tmV, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.vpool, (uint64_t)slots, (uint64_t)a.nkv * HD, (uint64_t)a.nkv * HD, kPage, 64);
     if (rc) return rc;
   }
   const size_t smem = TreeRing<HD, Q8, PAIR>::bytes;

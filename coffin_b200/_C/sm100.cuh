@@ -43,11 +43,6 @@ __device__ __forceinline__ void tma_load_2d(void* smem_dst, const void* tmap, ui
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1) : "memory");
 }
-__device__ __forceinline__ void tma_load_3d(void* smem_dst, const void* tmap, uint64_t* bar, int c0, int c1, int c2) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-      ::"r"(smem_u32(smem_dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2) : "memory");
-}
 // untiled: both addresses and the size are multiples of 16 bytes
 __device__ __forceinline__ void bulk_load(void* smem_dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -254,18 +249,6 @@ static inline cb_encode_tiled_fn cb_get_encode() {
       fn = (cb_encode_tiled_fn)p;
   }
   return fn;
-}
-// The same row-major bf16 tensor [rows, chunks * 64] as [chunks][rows][64]: one copy brings box_chunks pieces of 64 columns of box_rows rows,
-// each with 128B swizzle, one after the other.
-static inline int cb_make_tmap_chunks(CUtensorMap* map, const void* base, uint64_t rows, uint64_t chunks, uint32_t box_rows, uint32_t box_chunks) {
-  cb_encode_tiled_fn enc = cb_get_encode();
-  if (!enc) return CB_ERR_DRIVER;
-  if ((uintptr_t)base & 15) return CB_ERR_SHAPE;
-  cuuint64_t dims[3] = {64, rows, chunks}, strides[2] = {chunks * 128, 128};
-  cuuint32_t box[3] = {64, box_rows, box_chunks}, estr[3] = {1, 1, 1};
-  CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? 0 : CB_ERR_DRIVER;
 }
 // 2-D row-major tensor [rows, cols] of `esize`-byte elements, box [box_rows, box_cols], 128B swizzle.
 static inline int cb_make_tmap_2d(CUtensorMap* map, CUtensorMapDataType dt, int esize, const void* base,

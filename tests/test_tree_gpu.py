@@ -98,6 +98,18 @@ def test_attention_over_long_caches_of_uneven_length(q8):
     assert torch.equal(again, a.out), "the same inputs give the same bits"
 
 
+@pytest.mark.parametrize("q8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("R,C,nh,nkv,hd,longest", [(20, 33, 16, 4, 256, 900), (12, 64, 21, 7, 128, 1500), (43, 3, 16, 4, 256, 1200), (3, 64, 32, 4, 256, 3000),
+                                                   (150, 2, 4, 1, 64, 400), (2, 64, 16, 4, 256, 9000), (1, 43, 24, 4, 256, 5000)])
+def test_attention_of_pieces_that_hold_several_items_and_of_items_in_several_pieces(R, C, nh, nkv, hd, longest, q8):
+    """Many short sequences: pieces go on from one item to the next, with odd and even numbers of pages; few long ones: pieces end with them."""
+    rng = random.Random(R + C)
+    contexts = [rng.choice((0, 1, 64, rng.randrange(longest), rng.randrange(longest))) for _ in range(R - 1)] + [longest]
+    a = Attn(R, C, contexts, nh, nkv, hd, q8, "tree", seed=R + hd)
+    a.run()
+    a.check()
+
+
 def test_attention_skips_unused_rows_and_places():
     parents = [[-1, 0, None, 1, None], None, [-1, 0, 1, 2, 3]]
     a = Attn(3, 5, [100, -1, 31], 8, 2, 128, parents=parents, seed=5)
@@ -128,6 +140,41 @@ def test_attention_does_not_read_what_is_masked(q8):
             row = r * 6 + j
             if sick[r] not in P.path_of(a.parents[r], j):
                 assert torch.equal(a.out[row], healthy[row]), f"sequence {r} node {j} read a row that is not on its path"
+
+
+@pytest.mark.parametrize("q8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("hd", [128, 256])
+def test_attention_of_many_rows_does_not_read_what_is_masked(hd, q8):
+    """The same with more than 128 rows a kv head: behind a last page that is short, alone or the second of two, and of no tokens at all."""
+    contexts = [70, 128, 129, 0, 63]
+    a = Attn(5, 48, contexts, 8, 2, hd, q8, seed=9)
+    a.run()
+    a.check()
+    healthy = a.out.clone()
+    seen = torch.zeros(a.kpool.shape[0], dtype=torch.bool)
+    for r, ctx in enumerate(contexts):
+        seen[P.slots_of(a.tables[r].tolist(), range(ctx + 48))] = True
+    bad = (~seen).nonzero().flatten().cuda()
+    if q8:
+        a.kscale[bad], a.vscale[bad] = float("nan"), float("inf")
+    else:
+        a.kpool[bad], a.vpool[bad] = float("nan"), float("inf")
+    a.run()
+    assert torch.equal(a.out, healthy)
+
+
+def test_attention_of_many_rows_in_two_graphs_that_run_at_once():
+    a, b = (Attn(2, 64, [300, 1000], 16, 4, 256, seed=s) for s in (25, 26))
+    graphs = [_captured(x.run)[0] for x in (a, b)]
+    a.out.fill_(7.0), b.out.fill_(7.0)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+    torch.cuda.synchronize()
+    a.check(), b.check()
 
 
 def test_attention_with_strides_and_views():
