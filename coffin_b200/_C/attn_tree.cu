@@ -224,12 +224,31 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
   const bool lead = rank == 0;
   const int worker = blockIdx.x / HALF;
-  griddep_launch();
-  griddep_wait();
   if (smem_u32(smem_raw) & 1023) {
     if (threadIdx.x == 0) atomicCAS(a.status, 0, 89);
     return;
   }
+  // Tensor memory is taken before a later kernel may start beside this one: one that took it first would wait for this kernel with it.
+  if (warp == 1) {
+    if (PAIR) { tmem_alloc_pair(&tmem_base_s, TMEM_COLS); tmem_relinquish_pair(); }
+    else { tmem_alloc(&tmem_base_s, TMEM_COLS); tmem_relinquish(); }
+  } else if (warp == 2) {
+    if (lane == 0) {
+      abort_s = 0;
+      mbar_init(&q_full, 8 * HALF);
+      mbar_init(&o_full, 1);
+      mbar_init(&o_free, 8 * HALF);
+      for (int i = 0; i < 2 * ST; ++i) { mbar_init(&k_full[i], Q8 ? kLoaders / 64 * HALF : lead ? HALF : 1); mbar_init(&k_free[i], 1); }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4 * HALF); mbar_init(&p_full[i], 4 * HALF); mbar_init(&p_free[i], 1);
+      }
+      for (int i = 0; Q8 && i < SR; ++i) mbar_init(&sc_full[i], 2 * kPage);
+      for (int i = 0; i < 4; ++i) { mbar_init(&m_done[i][0], 1); mbar_init(&m_done[i][1], 1); mbar_init(&pair_bar[i], 64); }
+      mbar_fence_init();
+    }
+  }
+  griddep_launch();
+  griddep_wait();
   if (warp == 0) {
     int none, all;
     page_sums(a, 0, [](int n) { return n; }, &none, &all);
@@ -266,23 +285,6 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         const int p = L ? piece_start(i, n, k) : i;
         seg_s = Segments{L ? piece_start(i + 1, n, k) - p : hi - lo, r, n, it / a.tiles, it % a.tiles, r * per + it, 0, p};
       }
-    }
-  } else if (warp == 1) {                             // beside it
-    if (PAIR) { tmem_alloc_pair(&tmem_base_s, TMEM_COLS); tmem_relinquish_pair(); }
-    else { tmem_alloc(&tmem_base_s, TMEM_COLS); tmem_relinquish(); }
-  } else if (warp == 2) {
-    if (lane == 0) {
-      abort_s = 0;
-      mbar_init(&q_full, 8 * HALF);
-      mbar_init(&o_full, 1);
-      mbar_init(&o_free, 8 * HALF);
-      for (int i = 0; i < 2 * ST; ++i) { mbar_init(&k_full[i], Q8 ? kLoaders / 64 * HALF : lead ? HALF : 1); mbar_init(&k_free[i], 1); }
-      for (int i = 0; i < 2; ++i) {
-        mbar_init(&s_full[i], 1); mbar_init(&s_free[i], 4 * HALF); mbar_init(&p_full[i], 4 * HALF); mbar_init(&p_free[i], 1);
-      }
-      for (int i = 0; Q8 && i < SR; ++i) mbar_init(&sc_full[i], 2 * kPage);
-      for (int i = 0; i < 4; ++i) { mbar_init(&m_done[i][0], 1); mbar_init(&m_done[i][1], 1); mbar_init(&pair_bar[i], 64); }
-      mbar_fence_init();
     }
   }
   tc_fence_before();
