@@ -61,20 +61,6 @@ __device__ __forceinline__ int piece_of(int g, int T, int G) {
   const int q = T / G, rest = T % G, longer = rest * (q + 1);
   return g < longer ? g / (q + 1) : rest + (g - longer) / q;
 }
-// Sums over the sequences before `r` and over all of them, of f(pages of an item) (a warp)
-template <typename F>
-__device__ __forceinline__ void page_sums(const TreeAttnArgs& a, int r, const F& f, int* before, int* all) {
-  const int lane = threadIdx.x & 31;
-  int b = 0, t = 0;
-#pragma unroll 1
-  for (int i = lane; i < a.R; i += 32) {
-    const int n = f(cached_pages(a, i));
-    t += n;
-    if (i < r) b += n;
-  }
-  *before = __reduce_add_sync(0xffffffffu, b);
-  *all = __reduce_add_sync(0xffffffffu, t);
-}
 // Pages of a piece if no piece is to hold pages of two items: the smallest L for which ceil(n / L) pieces an item are no more than the
 // workers.  0 where it is kSwitch pages or more above an even share: going from one item to the next costs a worker about as long as
 // kSwitch pages (the sums leave tensor memory, the next Q enters it, and the chain of products starts anew).  us of a pass with whole
@@ -250,8 +236,10 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
   griddep_launch();
   griddep_wait();
   if (warp == 0) {
-    int none, all;
-    page_sums(a, 0, [](int n) { return n; }, &none, &all);
+    int all = 0;
+#pragma unroll 1
+    for (int i = lane; i < a.R; i += 32) all += cached_pages(a, i);
+    all = __reduce_add_sync(0xffffffffu, all);
     const int per = a.nkv * a.tiles, T = all * per, G = min(a.workers, T);
     const int L = T > G ? whole_pieces(a.positions, a.R, a.width, a.workers, T, per) : 0;      // (one page each: nothing to cut)
     if (blockIdx.x == 0 && lane == 0) *a.part_pages = L;
@@ -768,35 +756,31 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
   const int lane = threadIdx.x & 31;
   if (task >= (int64_t)a.R * a.C * a.nh) return;
   const int h = (int)(task % a.nh), j = (int)(task / a.nh % a.C), r = (int)(task / ((int64_t)a.nh * a.C));
-  const int pos0 = a.positions[r], L = *a.part_pages;
-  uint64_t on = (uint64_t)a.anc[(int64_t)r * a.C + j];
-  if (on == 0 || pos0 < 0) return;
-  on = (on & (~0ull >> (63 - j))) | 1ull << j;              // a path ends at its node
-  const int kvh = h / a.rep;
+  // what depends on nothing is requested first, then what depends on it: tables and the partials' maxima, then rows
   const int64_t row = (int64_t)r * a.C + j;
-  float q[EPL], o[EPL];
+  const int pos0 = a.positions[r], L = *a.part_pages, mine0 = lane < a.R ? a.positions[lane] : -1;
+  uint64_t on = (uint64_t)a.anc[row];
   RowPiece<EPL, false> qp, gp;
   qp.load(a.q, (row * a.nh + h) * HD + lane * EPL);
   if (a.gate) gp.load(a.gate, row * a.ldg + (int64_t)h * 2 * HD + HD + lane * EPL);
+  if (on == 0 || pos0 < 0) return;
+  on = (on & (~0ull >> (63 - j))) | 1ull << j;              // a path ends at its node
+  const int kvh = h / a.rep;
+  int64_t slot0[2];
 #pragma unroll
-  for (int e = 0; e < EPL; ++e) { q[e] = qp.at(e) * a.scale_log2; o[e] = 0.f; }
-  // pool rows of the path; a page that is none takes its nodes off it
-  int64_t kr[2];
-  float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
-  uint64_t path = 0;
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int i = lane + 32 * u, p = pos0 + i;
-    const bool mine = on >> i & 1;
-    const int64_t slot0 = mine ? page_slot(a, r, p / kPage) : -1;
-    kr[u] = slot0 < 0 ? 0 : (slot0 + p % kPage) * a.nkv + kvh;
-    if (Q8 && slot0 >= 0) { ks[u] = a.kscale[kr[u]]; vs[u] = a.vscale[kr[u]]; }
-    path |= (uint64_t)__ballot_sync(0xffffffffu, slot0 >= 0) << (32 * u);
-  }
+  for (int u = 0; u < 2; ++u) slot0[u] = on >> (lane + 32 * u) & 1 ? page_slot(a, r, (pos0 + lane + 32 * u) / kPage) : -1;
   // the cache's partials: maxima and sums, one a lane
-  int before, all;
-  page_sums(a, r, [L](int n) { return L ? (n + L - 1) / L : n; }, &before, &all);
-  const int n = cached_pages(a, r), per = a.nkv * a.tiles, lrow = j * a.rep + h % a.rep, it = kvh * a.tiles + lrow / a.span, item = r * per + it;
+  auto pieces = [&](int pos) { const int n = pages_of(pos, a.width); return L ? (n + L - 1) / L : n; };
+  int all = pieces(mine0), before = lane < r ? all : 0;
+#pragma unroll 1
+  for (int i = lane + 32; i < a.R; i += 32) {
+    const int x = pieces(a.positions[i]);
+    all += x;
+    if (i < r) before += x;
+  }
+  all = __reduce_add_sync(0xffffffffu, all);
+  before = __reduce_add_sync(0xffffffffu, before);
+  const int n = pages_of(pos0, a.width), per = a.nkv * a.tiles, lrow = j * a.rep + h % a.rep, it = kvh * a.tiles + lrow / a.span, item = r * per + it;
   int b0 = 0, parts = 0;
   if (n > 0 && L) {
     parts = (n + L - 1) / L;
@@ -807,9 +791,24 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
     parts = piece_of(g0 + n - 1, T, G) - b0 + 1;
   }
   const int64_t at0 = (int64_t)(b0 + item) * a.used + lrow % a.span;
-  float m = -INFINITY, l = 0.f;
+  auto sums = [&](int b) { return b < parts ? *reinterpret_cast<const float2*>(a.part_ml + (at0 + (int64_t)b * a.used) * 2) : make_float2(-INFINITY, 0.f); };
+  const float2 ml0 = sums(lane);
+  // pool rows of the path; a page that is none takes its nodes off it
+  int64_t kr[2];
+  float ks[2] = {1.f, 1.f}, vs[2] = {1.f, 1.f};
+  uint64_t path = 0;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    kr[u] = slot0[u] < 0 ? 0 : (slot0[u] + (pos0 + lane + 32 * u) % kPage) * a.nkv + kvh;
+    if (Q8 && slot0[u] >= 0) { ks[u] = a.kscale[kr[u]]; vs[u] = a.vscale[kr[u]]; }
+    path |= (uint64_t)__ballot_sync(0xffffffffu, slot0[u] >= 0) << (32 * u);
+  }
+  float q[EPL], o[EPL];
+#pragma unroll
+  for (int e = 0; e < EPL; ++e) { q[e] = qp.at(e) * a.scale_log2; o[e] = 0.f; }
+  float m = ml0.x, l = 0.f;
 #pragma unroll 1
-  for (int b = lane; b < parts; b += 32) m = fmaxf(m, a.part_ml[(at0 + (int64_t)b * a.used) * 2]);
+  for (int b = lane + 32; b < parts; b += 32) m = fmaxf(m, sums(b).x);
   m = warp_max(m);
   // the path, kAtOnce nodes at a time: keys and values are requested together
 #pragma unroll 1
@@ -862,12 +861,9 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
   const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll 1
   for (int c = 0; c < parts; c += 32) {
-    float f = 0.f;
-    if (c + lane < parts) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (at0 + (int64_t)(c + lane) * a.used) * 2);
-      f = exp2f(ml.x - ms);                                 // 0 where these pages hold no key
-      l += f * ml.y;
-    }
+    const float2 ml = c ? sums(c + lane) : ml0;
+    const float f = exp2f(ml.x - ms);                       // 0 where these pages hold no key
+    l += f * ml.y;
     const int here = min(32, parts - c);
 #pragma unroll 1
     for (int b = 0; b < here; b += kAtOnce) {
