@@ -8,8 +8,8 @@
 // convolution along the path: its older taps are the node's ancestors, behind them the ring.  State and ring stay as they were; k, d and
 // alpha of every node are recorded and the raw rows kept, from which a commit replays the accepted path (tree_commit.cu).
 //
-// 1. rows: a warp a (node, head) convolves, norms q and k and leaves them, and v, as fp32 rows by head.  (Within the kernel below it was
-//    repeated for every value head of a key head and every group of columns.)
+// 1. rows: a warp a (node, head) convolves, norms q and k and leaves them, and v, as fp32 rows by head.  (Within the kernel below it would be
+//    repeated for every value head of a key head and every group of columns, which only few nodes are worth.)
 // 2. nodes: a CTA owns DVS columns of one head's state; the DV / DVS CTAs of a head are a cluster, share out the Gram matrices and
 //    exchange the sums of squares of the norm.  (1 - A)^-1 of the strictly lower matrix A of the first equation is built from inverted 8 x 8
 //    blocks by doubling, so that what follows are small dense products.
@@ -21,7 +21,7 @@
 
 namespace {
 
-constexpr int kRing = 16, kMaxNodes = 64, kThreads = 256;
+constexpr int kRing = 16, kMaxNodes = 64, kThreads = 256, kFuse = 8;
 
 struct GdnTreeArgs {
   const bf16* proj; int64_t ldp;          // [R * C, ldp]: q | k | v | z | b | a
@@ -48,17 +48,11 @@ __device__ __forceinline__ bool unused(const GdnTreeArgs& a, int r) {
 }
 
 // ---- rows -----------------------------------------------------------------------------------
+// Four (two) channels a lane of head u's row at node j: convolved along the path `on`, SiLU, q and k normed.  `raw` says whether to keep the raw row.
 template <int D>
-__global__ void __launch_bounds__(kThreads) gdn_tree_rows_kernel(const GdnTreeArgs a) {
+__device__ __forceinline__ void tree_row(const GdnTreeArgs& a, int r, int j, uint64_t on, int u, bool raw, float (&y)[D / 32]) {
   constexpr int E = D / 32;
-  griddep_launch();
-  griddep_wait();
-  const int heads = 2 * a.nk + a.nv, lane = threadIdx.x & 31;
-  const int u = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), j = blockIdx.y, r = blockIdx.z;
-  if (u >= heads) return;
-  const uint64_t on = path_word(a, r, j);
-  if (on == 0 || unused(a, r)) return;
-  const int conv = heads * D, c = u * D + lane * E, pos = a.positions[r] + __popcll(on) - 1;
+  const int lane = threadIdx.x & 31, conv = (2 * a.nk + a.nv) * D, c = u * D + lane * E, pos = a.positions[r] + __popcll(on) - 1;
   const bf16* ring = a.ring + (int64_t)a.slots[r] * kRing * conv + c;
   const bf16* rows = a.proj + (int64_t)r * a.C * a.ldp + c;
   uint32_t x[4][E / 2];
@@ -75,18 +69,22 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_rows_kernel(const GdnTreeAr
       else x[b][0] = *reinterpret_cast<const uint32_t*>(from);
     }
   }
-  bf16* raw = a.raw + ((int64_t)r * a.C + j) * conv + c;
-  if (E == 4) *reinterpret_cast<uint2*>(raw) = *reinterpret_cast<const uint2*>(x[0]);
-  else *reinterpret_cast<uint32_t*>(raw) = x[0][0];
-  float y[E], ss = 0.f;
+  float4 w[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) w[e] = *reinterpret_cast<const float4*>(a.conv_w + (int64_t)(c + e) * 4);
+  if (raw) {
+    bf16* to = a.raw + ((int64_t)r * a.C + j) * conv + c;
+    if (E == 4) *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(x[0]);
+    else *reinterpret_cast<uint32_t*>(to) = x[0][0];
+  }
+  float ss = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) {
-    const float4 w = *reinterpret_cast<const float4*>(a.conv_w + (int64_t)(c + e) * 4);
     const auto f = [&](int b) { return __uint_as_float(e & 1 ? x[b][e / 2] & 0xffff0000u : x[b][e / 2] << 16); };
-    float v = w.x * f(3);
-    v = fmaf(w.y, f(2), v);
-    v = fmaf(w.z, f(1), v);
-    v = fmaf(w.w, f(0), v);
+    float v = w[e].x * f(3);
+    v = fmaf(w[e].y, f(2), v);
+    v = fmaf(w[e].z, f(1), v);
+    v = fmaf(w[e].w, f(0), v);
     y[e] = v / (1.f + expf(-v));
     ss = fmaf(y[e], y[e], ss);
   }
@@ -96,6 +94,20 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_rows_kernel(const GdnTreeAr
 #pragma unroll
     for (int e = 0; e < E; ++e) y[e] *= f;
   }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) gdn_tree_rows_kernel(const GdnTreeArgs a) {
+  constexpr int E = D / 32;
+  griddep_launch();
+  griddep_wait();
+  const int heads = 2 * a.nk + a.nv, lane = threadIdx.x & 31;
+  const int u = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), j = blockIdx.y, r = blockIdx.z;
+  if (u >= heads) return;
+  const uint64_t on = path_word(a, r, j);
+  if (on == 0 || unused(a, r)) return;
+  float y[E];
+  tree_row<D>(a, r, j, on, u, true, y);
   float* to = a.rows + (((int64_t)r * heads + u) * a.C + j) * D + lane * E;
   if (E == 4) *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(y);
   else *reinterpret_cast<float2*>(to) = *reinterpret_cast<const float2*>(y);
@@ -163,7 +175,7 @@ __device__ __forceinline__ void sync_all() {
   else __syncthreads();
 }
 
-template <int DK, int DV, int DVS, bool TILE>
+template <int DK, int DV, int DVS, bool TILE, bool FUSE>
 __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a) {
   constexpr int NS = DV / DVS, LK = TreeSmem<DK, DVS, TILE>::LK;
   extern __shared__ __align__(16) float sm[];
@@ -193,7 +205,7 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a)
     xa = __bfloat162float(row[a.nv + h]);
   }
   const float rate = a.A_log[h], dtb = a.dt_bias[h];
-  {
+  if (!FUSE) {
     const float* q = a.rows + ((int64_t)r * heads + kh) * C * DK;
     const float* k = q + (int64_t)a.nk * C * DK;
     const float* v = a.rows + ((int64_t)r * heads + 2 * a.nk + h) * C * DV + col0;
@@ -208,6 +220,8 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a)
       const int j = i / (DVS / 4), c = i % (DVS / 4) * 4;
       copy16(d + j * DVS + c, v + (int64_t)j * DV + c);
     }
+  }
+  {
     const bf16* z = a.proj + (int64_t)r * C * a.ldp + conv + h * DV + col0;
 #pragma unroll 1
     for (int i = tid; i < C * DVS / 8; i += kThreads) {
@@ -234,6 +248,22 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a)
       if (WC == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(sp + k * DV);
       else if (WC == 2) *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(sp + k * DV);
       else x[0] = sp[k * DV];
+    }
+  }
+  if (FUSE) {                                                // a warp a row of q, k or v
+#pragma unroll 1
+    for (int i = warp; i < 3 * C; i += kThreads / 32) {
+      const int j = i / 3, which = i % 3, u = which == 0 ? kh : which == 1 ? a.nk + kh : 2 * a.nk + h;
+      const uint64_t path = path_word(a, r, j);
+      if (path == 0) continue;
+      float y[DK / 32];
+      tree_row<DK>(a, r, j, path, u, cg == 0 && (which == 2 || h % a.rep == 0), y);
+      const int c = lane * (DK / 32) - (which == 2 ? col0 : 0);        // (DK = DV)
+      float* to = which == 0 ? qn + j * LK + c : which == 1 ? kn + j * LK + c : d + j * DVS + c;
+      if (c >= 0 && (which < 2 || c < DVS)) {
+        if (DK == 128) *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(y);
+        else *reinterpret_cast<float2*>(to) = *reinterpret_cast<const float2*>(y);
+      }
     }
   }
   if (tid < Cp) {
@@ -540,9 +570,9 @@ __global__ void __launch_bounds__(kThreads) gdn_tree_kernel(const GdnTreeArgs a)
   }
 }
 
-template <int DK, int DV, int DVS, bool TILE = false>
+template <int DK, int DV, int DVS, bool FUSE, bool TILE = false>
 int launch_gdn_tree(const GdnTreeArgs& a, int R, cudaStream_t st) {
-  auto kern = gdn_tree_kernel<DK, DV, DVS, TILE>;
+  auto kern = gdn_tree_kernel<DK, DV, DVS, TILE, FUSE>;
   const size_t smem = TreeSmem<DK, DVS, TILE>(a.Cp).total * sizeof(float);
   static SmemLimit limit;
   std::lock_guard<std::mutex> lock(limit.held);
@@ -554,12 +584,19 @@ int launch_gdn_tree(const GdnTreeArgs& a, int R, cudaStream_t st) {
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = DV / DVS; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  int n = 0;
+  if (g_cb_use_pdl) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (DV / DVS > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = DV / DVS;
+    attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+    ++n;
+  }
   cfg.attrs = attr;
-  cfg.numAttrs = g_cb_use_pdl ? 2 : 1;
+  cfg.numAttrs = (unsigned)n;
   if (g_cb_trace_names) cb_trace_name((const void*)kern);
   return (int)cudaLaunchKernelEx(&cfg, kern, a);
 }
@@ -570,7 +607,7 @@ CB_EXPORT int cb_gdn_tree(const void* proj, int64_t ldp, const void* conv_w, con
                           const void* ring, const void* state, const void* slots, const void* positions, const void* anc, void* out, int64_t ldo,
                           void* record, void* raw, void* rows, int64_t nslots, int64_t R, int64_t C, int64_t nk, int64_t nv, int64_t dk, int64_t dv, float eps,
                           int64_t gate_sigmoid, void* stream) {
-  if (!proj || !conv_w || !A_log || !dt_bias || !norm_w || !ring || !state || !slots || !positions || !anc || !out || !record || !raw || !rows) return CB_ERR_ARG;
+  if (!proj || !conv_w || !A_log || !dt_bias || !norm_w || !ring || !state || !slots || !positions || !anc || !out || !record || !raw) return CB_ERR_ARG;
   if (R < 1 || R > 65535 || C < 1 || C > kMaxNodes || nk < 1 || nv < 1 || nv % nk || nv > 65535 || ldp % 8 || ldo % 4 || ((uintptr_t)out & 7) || ((uintptr_t)norm_w & 15) ||
       (((uintptr_t)proj | (uintptr_t)ring | (uintptr_t)state | (uintptr_t)raw | (uintptr_t)rows | (uintptr_t)conv_w) & 15)) return CB_ERR_SHAPE;
   GdnTreeArgs a{(const bf16*)proj, ldp, (const float*)conv_w, (const float*)A_log, (const float*)dt_bias, (const float*)norm_w, (const bf16*)ring,
@@ -578,15 +615,23 @@ CB_EXPORT int cb_gdn_tree(const void* proj, int64_t ldp, const void* conv_w, con
                 (int)R, (int)C, (int)((C + 7) / 8 * 8), (int)nk, (int)nv, (int)(nv / nk), (int)nslots, (int)gate_sigmoid, eps};
   cudaStream_t st = (cudaStream_t)stream;
   if (!((dk == 128 && dv == 128) || (dk == 64 && dv == 64))) return CB_ERR_SHAPE;
-  const dim3 grid((unsigned)((2 * nk + nv + kThreads / 32 - 1) / (kThreads / 32)), (unsigned)C, (unsigned)R);
-  cudaError_t e = dk == 128 ? cb_launch(gdn_tree_rows_kernel<128>, grid, dim3(kThreads), 0, st, a) : cb_launch(gdn_tree_rows_kernel<64>, grid, dim3(kThreads), 0, st, a);
-  if (e != cudaSuccess) return (int)e;
+  // Few nodes: the rows in the kernel that uses them, repeated for the value heads of a key head, a launch less.  us of a pass with a kernel
+  // of their own / without: 4 nodes, 32 heads 11.5 / 11.2, 8 x 4 nodes 16.1 / 14.4, 8 x 8 nodes 16.8 / 16.5, 4 x 12 nodes, 48 heads 22.9 / 24.4,
+  // 8 x 16 nodes 25.7 / 27.3; a call's host time 18 / 14.
+  const bool fuse = C <= kFuse;
+  if (!fuse && !rows) return CB_ERR_ARG;
+  if (!fuse) {
+    const dim3 grid((unsigned)((2 * nk + nv + kThreads / 32 - 1) / (kThreads / 32)), (unsigned)C, (unsigned)R);
+    cudaError_t e = dk == 128 ? cb_launch(gdn_tree_rows_kernel<128>, grid, dim3(kThreads), 0, st, a) : cb_launch(gdn_tree_rows_kernel<64>, grid, dim3(kThreads), 0, st, a);
+    if (e != cudaSuccess) return (int)e;
+  }
   // A head's columns are split over a cluster while all CTAs still run at once.  us of 1 / 2 / 4 CTAs a head: 16 nodes, 32 heads 21.1 / 18.0 /
   // 17.9, 128 heads 23.9 / 20.9 / 32.6, 256 heads 25.6 / 35.4 / 47.2; 64 nodes, 32 heads 49.9 / 36.0 / 30.3, 192 heads 106.7 / 106.4 / 156.4.
-  // Up to eight nodes the exchange costs more than it saves: 4 nodes, 32 heads 11.8 / 12.8 / 13.3.
+  // Up to eight nodes the exchange costs more than it saves: 4 nodes, 32 heads 11.8 / 12.8 / 13.3 (128-wide heads; those of 64 have two CTAs throughout).
   const int64_t room = 148 / (R * nv);
-  const int ns = C <= 8 || room < 2 ? 1 : (room < 4 ? 2 : 4);
-  if (dk == 128 && ns == 1 && C > 48) return launch_gdn_tree<128, 128, 128, true>(a, (int)R, st);
-  if (dk == 128) return ns == 1 ? launch_gdn_tree<128, 128, 128>(a, (int)R, st) : ns == 2 ? launch_gdn_tree<128, 128, 64>(a, (int)R, st) : launch_gdn_tree<128, 128, 32>(a, (int)R, st);
-  return launch_gdn_tree<64, 64, 32>(a, (int)R, st);              // two CTAs a head
+  const int ns = fuse || room < 2 ? 1 : (room < 4 ? 2 : 4);
+  if (fuse) return dk == 128 ? launch_gdn_tree<128, 128, 128, true>(a, (int)R, st) : launch_gdn_tree<64, 64, 32, true>(a, (int)R, st);
+  if (dk == 64) return launch_gdn_tree<64, 64, 32, false>(a, (int)R, st);              // two CTAs a head
+  if (ns == 1 && C > 48) return launch_gdn_tree<128, 128, 128, false, true>(a, (int)R, st);
+  return ns == 1 ? launch_gdn_tree<128, 128, 128, false>(a, (int)R, st) : ns == 2 ? launch_gdn_tree<128, 128, 64, false>(a, (int)R, st) : launch_gdn_tree<128, 128, 32, false>(a, (int)R, st);
 }

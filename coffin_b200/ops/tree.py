@@ -178,10 +178,10 @@ def gdn_tree(proj, conv_w, A_log, dt_bias, norm_w, ring, state, slots, positions
     recp, rawp = _vec(record, nodes * nv * (dk + dv + 1), _F32, "record"), _vec(raw, nodes * conv, _BF, "raw", 16)
     i = _place(proj, conv_w, A_log, dt_bias, norm_w, ring, state, slots, positions, anc, out, record, raw)
     if R:
-        rows = torch.empty(nodes * conv, dtype=_F32, device=proj.device)
-        call("gdn_tree", i, pp, ldp, wp, Ap, bp, np_, rp, sp, slp, posp, anc.data_ptr(), op, ldo, recp, rawp, rows.data_ptr(), n, R, C, nk, nv, dk, dv,
+        rows = torch.empty(nodes * conv, dtype=_F32, device=proj.device) if C > 8 else None      # few nodes: one kernel
+        call("gdn_tree", i, pp, ldp, wp, Ap, bp, np_, rp, sp, slp, posp, anc.data_ptr(), op, ldo, recp, rawp, 0 if rows is None else rows.data_ptr(), n, R, C, nk, nv, dk, dv,
              float(eps), int(gate_sigmoid))
-        K._count(2)
+        K._count(1 if rows is None else 2)
     return out
 
 
