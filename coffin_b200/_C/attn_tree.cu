@@ -946,7 +946,7 @@ int launch_tree(const TreeAttnArgs& a, int64_t slots, cudaStream_t st) {
   else rc = launch_cache<HD, Q8, false>(a, slots, st);
   if (rc) return rc;
   const int64_t tasks = (int64_t)a.R * a.C * a.nh;
-  return (int)cb_launch(tree_finish_kernel<HD, Q8>, dim3((unsigned)((tasks + 7) / 8)), dim3(256), 0, st, a);
+  return (int)cb_launch_second(tree_finish_kernel<HD, Q8>, dim3((unsigned)((tasks + 7) / 8)), dim3(256), 0, st, a);
 }
 
 }  // namespace

@@ -77,7 +77,7 @@ __device__ __forceinline__ void griddep_launch() {
 extern int g_cb_use_pdl;
 
 template <typename... KArgs, typename... Args>
-static inline cudaError_t cb_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
+static inline cudaError_t cb_launch_pdl(bool pdl, void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
                                     cudaStream_t stream, Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -88,9 +88,19 @@ static inline cudaError_t cb_launch(void (*kernel)(KArgs...), dim3 grid, dim3 bl
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = g_cb_use_pdl ? 1 : 0;
+  cfg.numAttrs = pdl ? 1 : 0;
   if (g_cb_trace_names) cb_trace_name((const void*)kernel);
   return cudaLaunchKernelEx(&cfg, kernel, KArgs(args)...);
+}
+template <typename... KArgs, typename... Args>
+static inline cudaError_t cb_launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+  return cb_launch_pdl(g_cb_use_pdl, kernel, grid, block, smem, stream, args...);
+}
+// The second kernel of an operator that consists of two: it may come up beside the first whatever the switch says, which concerns
+// kernels of different operators.  (2 to 6 us a call where launches are plain.)
+template <typename... KArgs, typename... Args>
+static inline cudaError_t cb_launch_second(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+  return cb_launch_pdl(true, kernel, grid, block, smem, stream, args...);
 }
 
 // The same with a preferred split of the SM's memory between L1 and shared memory: `carve` percent shared.  Loads in flight

@@ -520,7 +520,7 @@ CB_EXPORT int cb_verify_tree(const void* logits, int64_t lds, int64_t ldr, const
   a.arrived = (unsigned*)(a.picks + R * C);
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e = cb_launch(row_stats_kernel, dim3((unsigned)((a.P + kNT / 32 - 1) / (kNT / 32)), (unsigned)(R * C)), dim3(kNT), 0, st, a);
-  if (e == cudaSuccess) e = cb_launch(tree_pick_kernel, dim3((unsigned)(R * C)), dim3(kNT), 0, st, a);
+  if (e == cudaSuccess) e = cb_launch_second(tree_pick_kernel, dim3((unsigned)(R * C)), dim3(kNT), 0, st, a);
   return (int)e;
 }
 
@@ -539,6 +539,6 @@ CB_EXPORT int cb_verify_drafts(const void* logits, int64_t lds, int64_t ldr, con
   a.arrived = (unsigned*)(a.rest + R * a.P);
   cudaStream_t st = (cudaStream_t)stream;
   cudaError_t e = cb_launch(row_stats_kernel, dim3((unsigned)((a.P + kNT / 32 - 1) / (kNT / 32)), (unsigned)(R * C)), dim3(kNT), 0, st, a);
-  if (e == cudaSuccess) e = cb_launch(draft_rest_kernel, dim3((unsigned)a.P, (unsigned)R), dim3(kNT), 0, st, a);
+  if (e == cudaSuccess) e = cb_launch_second(draft_rest_kernel, dim3((unsigned)a.P, (unsigned)R), dim3(kNT), 0, st, a);
   return (int)e;
 }

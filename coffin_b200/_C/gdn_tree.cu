@@ -585,7 +585,7 @@ int launch_gdn_tree(const GdnTreeArgs& a, int R, cudaStream_t st) {
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   int n = 0;
-  if (g_cb_use_pdl) {
+  if (g_cb_use_pdl || !FUSE) {                               // (behind the rows, it is the second kernel of the operator)
     attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[n++].val.programmaticStreamSerializationAllowed = 1;
   }
