@@ -8,9 +8,14 @@
 // keys are few and sparse: a warp walks the set bits of a row and merges the partial sums of the cache.  A key that is not on a node's
 // path is never multiplied, whatever it holds, and values behind the cache's end are cleared before they are.
 //
-// Cache kernel: an item is (sequence, kv head, 128 rows); the pages of all items form one list that the CTAs, one an SM, cut into even
-// pieces, whatever the lengths.  A CTA walks the segments of its piece; each leaves unnormalised sums, maxima and sums of weights in
-// slot (CTA + item), which is different for any two segments because one of the two grows from segment to segment.
+// Cache kernel: an item is (sequence, kv head, 128 rows); the pages of all items form one list that the CTAs, one an SM, cut into pieces of
+// the same length, whatever the sequences'.  A CTA walks the segments of its piece; each leaves unnormalised sums, maxima and sums of
+// weights in slot (CTA + item), which is different for any two segments because one of the two grows from segment to segment.
+// More than 128 rows a kv head: an item has 256, of which each CTA of a pair (cta_group::2) holds half.  Both bring half the bytes of every
+// page, the even one issues the products, and what those threads wait for is signalled there by both.  (Two items of 128 rows bring every
+// page twice: 2 x 64 nodes behind 65536 tokens 193 us, in pairs 149.)
+// What bounds it: 8 x 16 nodes behind 517 to 16391 tokens, 280 MB in 52 us, 5.4 TB/s, the rest are the ends of the pieces and the merge; 2 x 64
+// nodes behind 65536 tokens, 540 MB and 137 GFLOP in 110 us, tensor pipe 67 % busy; int8 pages, the issue slots that softmax and conversion share.
 //   warp 0       TMA: K and V pages into rings (a page of a kv head is a [64 x hd] box of the pool, hd / 64 swizzled [64 x 128 B] blocks)
 //   warp 1, 10   tcgen05.mma (one thread each): S = Q K^T with Q in tensor memory into one of two accumulators; O += P V
 //   warps 2-9    two groups of 128 threads, a thread a row: one takes the even pages, the other the odd ones, so that the exponentials of a
@@ -183,7 +188,7 @@ __global__ void __launch_bounds__(Q8 ? 352 + kLoaders : 352, 1)
 tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeAttnArgs a) {
   // bf16 pairs take two pages a step: a page of K each, the two sides of one product of 128 keys (products of 64 keys take 46 cycles per 16
   // channels, of 128 keys 64 cycles), and half the channels of V of both.  An odd last page has a partner that is none.
-  constexpr bool TWO = PAIR && !Q8, HOLD = TWO;
+  constexpr bool TWO = PAIR && !Q8;
   constexpr int HALF = PAIR ? 2 : 1, STEP = TWO ? 2 : 1, NC = HD / 64, VC = NC / HALF, ST = TreeRing<HD, Q8, PAIR>::stages, SPAN = kRows * HALF;
   // Scales of an int8 page are read until its accumulator is free.  K of page n is converted after the scores of page n - ST, and those
   // were multiplied after the accumulator of page n - ST - 2 was free.
@@ -553,16 +558,16 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         // Two pages a product: the scores go to registers whole, and the accumulators are free for the next product before any exponential
         // (2 x 64 nodes behind 65536 tokens 131 us, freed behind them 174).  Else 32 columns at a time, and twice, which leaves half the
         // registers and half the code (8 x 16 nodes behind up to 16391 tokens 64.1 us, whole 65.6).
-        uint32_t sv[HOLD ? kPage : 32];
+        uint32_t sv[TWO ? kPage : 32];
         auto scores = [&](int c0) {
           tmem_ld32(tmem_base + lane_base + sb * kPage + c0, sv);
-          if (HOLD) tmem_ld32(tmem_base + lane_base + sb * kPage + 32, sv + (HOLD ? 32 : 0));
+          if (TWO) tmem_ld32(tmem_base + lane_base + sb * kPage + 32, sv + (TWO ? 32 : 0));
           tmem_ld_wait();
         };
         auto mask = [&](int c0) {                     // (int8: scales behind the end are 1)
           if (valid < kPage) {
 #pragma unroll
-            for (int c = 0; c < (HOLD ? kPage : 32); ++c)
+            for (int c = 0; c < (TWO ? kPage : 32); ++c)
               if (c0 + c >= valid) sv[c] = __float_as_uint(-INFINITY);
           }
         };
@@ -572,16 +577,16 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
         if (!idle) {
           float mx1 = -INFINITY;
 #pragma unroll 1
-          for (int c0 = 0; c0 < kPage; c0 += HOLD ? kPage : 32) {
+          for (int c0 = 0; c0 < kPage; c0 += TWO ? kPage : 32) {
             scores(c0);
-            if (HOLD) {
+            if (TWO) {
               tc_fence_before();
               __syncwarp();
               if (lane == 0) signal(&s_free[sb]);
             }
             mask(c0);
 #pragma unroll
-            for (int c = 0; c < (HOLD ? kPage : 32); c += 2) {
+            for (int c = 0; c < (TWO ? kPage : 32); c += 2) {
               float s0 = __uint_as_float(sv[c]), s1 = __uint_as_float(sv[c + 1]);
               if (Q8) unpack2(mul2(pack2(s0, s1), ks2[(c0 + c) / 2]), s0, s1);
               mx = fmaxf(mx, s0);
@@ -590,7 +595,7 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           }
           mx = fmaxf(mx, mx1);
           if (!Q8) mx *= a.scale_log2;
-        } else if (HOLD && lane == 0) signal(&s_free[sb]);
+        } else if (TWO && lane == 0) signal(&s_free[sb]);
         if (p == seg.p0) m = mx;
         else {                                        // the other group has left the reference of the page before
           if (!tree_wait(&m_done[q][sb ^ 1], ((n - 1) >> 1) & 1, abort_flag)) { if (lane == 0) give_up(98); ok = false; break; }
@@ -631,13 +636,13 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           uint64_t l2 = 0;
           const uint64_t scale2 = pack2(a.scale_log2, a.scale_log2), minus2 = pack2(-ms, -ms);
 #pragma unroll 1
-          for (int c0 = 0; c0 < kPage; c0 += HOLD ? kPage : 32) {
-            if (!HOLD) {
+          for (int c0 = 0; c0 < kPage; c0 += TWO ? kPage : 32) {
+            if (!TWO) {
               scores(c0);
               mask(c0);
             }
 #pragma unroll
-            for (int c = 0; c < (HOLD ? 8 : 4); ++c) {
+            for (int c = 0; c < (TWO ? 8 : 4); ++c) {
               uint32_t pk[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -657,7 +662,7 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
           unpack2(l2, l0, l1);
           l += l0 + l1;
         }
-        if (!HOLD) {
+        if (!TWO) {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) signal(&s_free[sb]);
@@ -958,15 +963,17 @@ CB_EXPORT int cb_attn_tree(const void* q, const void* gate, int64_t ldg, const v
                            int64_t hd, void* status, void* stream) {
   if (!q || !kpool || !vpool || !tables || !positions || !anc || !out || !part || !status) return CB_ERR_ARG;
   if ((kscale == nullptr) != (vscale == nullptr)) return CB_ERR_ARG;
-  if (R < 1 || C < 1 || C > kMaxNodes || nkv < 1 || nh % nkv || ctas < 2 || ctas % 2 || ctas > 65534 || width < 1 || width > (1 << 24) || R * C * nh > (1ll << 30) || R * width * nkv * ((C * (nh / nkv) + kRows - 1) / kRows) > 0x7fffffff || slots > 0x7fffffff ||
-      ((uintptr_t)part & 15)) return CB_ERR_SHAPE;
+  if (R < 1 || C < 1 || C > kMaxNodes || nkv < 1 || nh < 1 || nh % nkv || ctas < 2 || ctas % 2 || ctas > 65534 || width < 1 || width > (1 << 24) ||
+      R * C * nh > (1ll << 30) || R * width * nkv * ((C * (nh / nkv) + kRows - 1) / kRows) > 0x7fff0000 || slots > 0x7fffffff || ((uintptr_t)part & 15))
+    return CB_ERR_SHAPE;
   // More than 128 rows a kv head: pairs of CTAs, each with half of every page.  (64 channels a head cannot be halved.)
   const int64_t rows = C * (nh / nkv), span = rows > kRows && hd >= 128 ? 2 * kRows : kRows, workers = span > kRows ? ctas / 2 : ctas;
   const int64_t tiles = (rows + span - 1) / span, used = rows < span ? rows : span;
   const int64_t places = (workers + R * nkv * tiles) * used;
   TreeAttnArgs a{(const bf16*)q, (const bf16*)gate, ldg, kpool, vpool, (const float*)kscale, (const float*)vscale, (const int*)tables, ldbt,
                  (int)width, (int)(slots / kPage), (const int*)positions, (const int64_t*)anc, (bf16*)out, ldo, (float*)part,
-                 (float*)part + places * hd, (int*)part + places * (hd + 2), (int)R, (int)C, (int)nh, (int)nkv, (int)(nh / nkv), (int)span, (int)tiles, (int)used, (int)workers,
+                 (float*)part + places * hd, (int*)part + places * (hd + 2), (int)R, (int)C, (int)nh, (int)nkv, (int)(nh / nkv), (int)span,
+                 (int)tiles, (int)used, (int)workers,
                  1.4426950408889634f / sqrtf((float)hd), (int*)status};
   cudaStream_t st = (cudaStream_t)stream;
   if (hd == 256) return kscale ? launch_tree<256, true>(a, slots, st) : launch_tree<256, false>(a, slots, st);

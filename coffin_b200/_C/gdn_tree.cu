@@ -626,7 +626,7 @@ CB_EXPORT int cb_gdn_tree(const void* proj, int64_t ldp, const void* conv_w, con
     if (e != cudaSuccess) return (int)e;
   }
   // A head's columns are split over a cluster while all CTAs still run at once.  us of 1 / 2 / 4 CTAs a head: 16 nodes, 32 heads 21.1 / 18.0 /
-  // 17.9, 128 heads 23.9 / 20.9 / 32.6, 256 heads 25.6 / 35.4 / 47.2; 64 nodes, 32 heads 49.9 / 36.0 / 30.3, 192 heads 106.7 / 106.4 / 156.4.
+  // 17.9, 128 heads 23.9 / 20.9 / 32.6, 256 heads 25.6 / 35.4 / 47.2; 64 nodes, 32 heads 49.9 / 36.0 / 30.3, 192 heads 93 (tiles) / 106.4 / 156.4.
   // Up to eight nodes the exchange costs more than it saves: 4 nodes, 32 heads 11.8 / 12.8 / 13.3 (128-wide heads; those of 64 have two CTAs throughout).
   const int64_t room = 148 / (R * nv);
   const int ns = fuse || room < 2 ? 1 : (room < 4 ? 2 : 4);
