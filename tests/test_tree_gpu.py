@@ -686,3 +686,32 @@ def test_a_verify_pass_of_trees_and_its_commit_equal_stepping_the_tokens(kind):
     tree.gdn_tree_commit(st.unsqueeze(0), rg.unsqueeze(0), chain.record.unsqueeze(0), chain.raw.unsqueeze(0), _i32(s.slots), _i32([pos0]),
                          _i32([list(range(n))]), _i32([n]))
     assert torch.equal(rg, ring) and (st - state).abs().max() <= 64 * n * P.U32 * state.abs().max()
+
+
+def test_calls_from_two_threads_on_streams_of_their_own():
+    """Launches that want different amounts of shared memory, from threads that do not wait for one another."""
+    import threading
+    jobs = [[Gdn(1, C, 4, 8, 128, [9], "tree", seed=40 + C) for C in (12, 40, 64)], [Attn(2, C, [300, 77], 8, 2, 128, C == 33, seed=50 + C) for C in (5, 33, 64)]]
+    failed = []
+
+    def work(mine):
+        try:
+            s = torch.cuda.Stream()
+            s.wait_stream(torch.cuda.default_stream())
+            with torch.cuda.stream(s):
+                for i in range(60):
+                    mine[i % len(mine)].run()
+            s.synchronize()
+        except Exception as e:          # noqa: BLE001
+            failed.append(e)
+
+    torch.cuda.synchronize()
+    threads = [threading.Thread(target=work, args=(m,)) for m in (jobs[0], jobs[0][::-1], jobs[1])]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for x in jobs[0] + jobs[1]:
+        x.check()
