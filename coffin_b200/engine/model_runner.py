@@ -350,7 +350,8 @@ class ModelRunner:
     # ------------------------------------------------------------------ trees of drafts
     @property
     def tree_capable(self) -> bool:
-        return hasattr(self.model, "verify_tree")
+        """Whether the model verifies trees as it is laid out (over several ranks it does not, and greedy rows draft chains)."""
+        return getattr(self.model, "verifies_trees", False)
 
     @property
     def tree_drafts(self) -> bool:

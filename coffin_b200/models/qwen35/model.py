@@ -1238,6 +1238,11 @@ class Qwen35Model:
     # ------------------------------------------------------------------ trees of drafts
     TREE_WIDTHS = (2, 4, 8, 16, 32, 64)
 
+    @property
+    def verifies_trees(self) -> bool:
+        """A verify pass over trees is single-GPU."""
+        return self.tp is None or (self.tp_world == 1 and self.ep_world == 1)
+
     def _tree_buffers(self, R: int, C: int) -> dict:
         b = self._verify_buffers(R, C)
         if "anc" not in b:
@@ -1266,7 +1271,7 @@ class Qwen35Model:
         N = R * C
         if N > BUCKETS[-1]:
             raise ValueError(f"{n} trees x {C} nodes exceed the {BUCKETS[-1]} token rows of one verify pass")
-        if self.tp is not None and (self.tp_world > 1 or self.ep_world > 1):
+        if not self.verifies_trees:
             raise NotImplementedError("a verify pass over trees is single-GPU")
         h_tok = torch.zeros(R, C, dtype=torch.int64)
         h_anc = torch.zeros(R, C, dtype=torch.int64)

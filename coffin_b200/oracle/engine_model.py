@@ -240,6 +240,8 @@ class OracleEngineModel:
                 cos, sin = O.mrope_cos_sin(pos.reshape(1, -1).expand(3, -1), c.rotary_dim, c.rope_theta, c.mrope_section)
                 self._forward(self.embed_tokens(torch.tensor(tokens[:n_accept])), pos0, slot, table, cos, sin)
 
+    verifies_trees = True
+
     @torch.no_grad()
     def verify_tree(self, rows: list[tuple]) -> torch.Tensor:
         """Logits ``[R, C, vocab]`` of trees of drafted tokens ``(tokens, parents, pos0, slot, block_table, rope_delta)``: the twin runs

@@ -1,0 +1,58 @@
+"""Which way a speculative step goes: trees where the model verifies them, chains where it does not."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+from coffin_b200.config import preset
+from coffin_b200.engine.config import EngineConfig
+from coffin_b200.engine.llm_engine import LLMEngine
+from coffin_b200.engine.sequence import SamplingParams
+from coffin_b200.oracle.engine_model import OracleEngineModel
+from coffin_b200.weights.init import random_state_dict
+
+CFG = preset("tiny")
+SD = random_state_dict(CFG, 0)
+
+
+class ChainsOnly(OracleEngineModel):
+    """What a model over several ranks is: it has the tree pass, but not for its layout."""
+    verifies_trees = False
+
+    def verify_tree(self, rows):
+        raise NotImplementedError("a verify pass over trees is single-GPU")
+
+
+def _engine(cls=OracleEngineModel, **kw):
+    return LLMEngine(cls(CFG, SD, max_seq=512, num_slots=4), EngineConfig(max_seq=512, max_num_seqs=4, graph=False, **kw))
+
+
+def _repetitive(seed: int, n: int = 60) -> list[int]:
+    g = torch.Generator().manual_seed(seed)
+    unit = torch.randint(0, CFG.vocab_size, (6,), generator=g).tolist()
+    return (unit * 20)[:n]
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("kw", [{"spec_tree": 7}, {"spec_sample": True}, {"spec_tree": 9, "spec_sample": True}])
+def test_a_model_without_tree_passes_drafts_chains(kw):
+    """Greedy rows draft chains, sampled ones do not draft, and all finish with the tokens of plain decoding."""
+    prompts = [_repetitive(1), _repetitive(2, 50)]
+    params = [SamplingParams(max_tokens=16), SamplingParams(max_tokens=16, temperature=0.05, seed=3)]
+    ref = [_engine().generate([p], q)[0].output for p, q in zip(prompts, params)]
+    eng = _engine(ChainsOnly, spec_k=3, spec_batch=True, **kw)
+    assert not eng.runner.tree_capable and not eng.runner.tree_drafts
+    seqs = [eng.add_request(p, q) for p, q in zip(prompts, params)]
+    assert eng.runner.spec_k_of(seqs[0]) == 3 and eng.runner.spec_k_of(seqs[1]) == 0
+    while any(not s.finished for s in seqs):
+        eng.step()
+    assert [s.output for s in seqs] == ref
+    assert seqs[0].spec_accepted > 0 and seqs[1].spec_drafted == 0
+
+
+def test_the_device_model_verifies_trees_on_one_rank_only():
+    from coffin_b200.models.qwen35.model import Qwen35Model
+    says = Qwen35Model.verifies_trees.fget
+    comm = object()
+    assert says(SimpleNamespace(tp=None, tp_world=1, ep_world=1)) and says(SimpleNamespace(tp=comm, tp_world=1, ep_world=1))
+    assert not says(SimpleNamespace(tp=comm, tp_world=2, ep_world=1)) and not says(SimpleNamespace(tp=comm, tp_world=1, ep_world=2))
