@@ -25,8 +25,9 @@ class EngineConfig:
     spec_batch: bool = False           # speculate also when several rows decode together (one verify pass over all rows)
     spec_tree: int = 0                 # drafted tokens a row may propose as a tree of continuations, up to spec_k deep (0 = one chain);
                                        # models without a verify pass over trees draft chains
-    spec_sample: bool = False          # requests with a temperature draft too: their own draws decide which drafts are kept, so that the
-                                       # tokens are those of plain sampling with the same seed (models with a verify pass over trees)
+    spec_sample: bool = False          # requests with a temperature draft too: their own draws decide which drafts are kept, so that what is
+                                       # drafted does not change their tokens (models with a verify pass over trees).  With this or spec_tree
+                                       # all draws are 64-bit; without, 32-bit, which gives another token in up to one of forty draws
     spec_min_ctx: int = 0              # rows shorter than this many tokens do not draft yet
     spec_sparse_k: int = 0             # approximate batched verify over the k best history blocks per row: accepted
                                        # as an option for parity with the reference, where it is also refused when

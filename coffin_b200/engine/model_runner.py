@@ -385,8 +385,9 @@ class ModelRunner:
         return trees if any(t for t, _p in trees) else None
 
     def tree_step(self, seqs: list[Sequence], tokens: list[int], trees: list[tuple[list[int], list[int]]]) -> list[list[int]]:
-        """One verify pass over every row's tree of drafts: the new tokens of each row, those that decoding token by token would give
-        (greedy, or drawn with the same uniforms of the row's generator).  States and pages advance by the accepted path."""
+        """One verify pass over every row's tree of drafts: the new tokens of each row, those that the steps without drafts would give
+        (greedy, or drawn as ``_sample`` draws, with the same uniforms of the row's generator).  States and pages advance by the
+        accepted path."""
         rows = [([tok] + list(d), [-1] + [p + 1 for p in par], s.num_computed, s.slot, s.blocks.table, s.rope_delta)
                 for s, tok, (d, par) in zip(seqs, tokens, trees)]
         self.model.verify_tree(rows)
@@ -486,7 +487,9 @@ class ModelRunner:
                 return [int(v) for v in greedy_tokens[:len(seqs)].tolist()]
             return [int(v) for v in self.model.sample(logits, None, None).tolist()]
         us = [self._generator(s).random() for s in seqs]
-        return [int(v) for v in self.model.sample(logits, temps, us).tolist()]
+        # beside tree steps, with their draw: a request's tokens do not depend on which of its steps drafted
+        draw = self.model.draw if self.tree_drafts else self.model.sample
+        return [int(v) for v in draw(logits, temps, us).tolist()]
 
     def _generator(self, seq: Sequence) -> random.Random:
         rng = self._rng.get(seq.seq_id)

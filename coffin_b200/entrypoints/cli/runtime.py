@@ -43,7 +43,7 @@ def parser() -> argparse.ArgumentParser:
     ap.add_argument("--spec-k", type=int, default=None)
     ap.add_argument("--spec-batch", action="store_true")
     ap.add_argument("--spec-tree", type=int, default=None, help="drafted tokens a row may propose as a tree of continuations, up to --spec-k deep (0: one chain)")
-    ap.add_argument("--spec-sample", action="store_true", help="requests with a temperature draft too; the tokens are those of plain sampling")
+    ap.add_argument("--spec-sample", action="store_true", help="requests with a temperature draft too; what is drafted does not change their tokens (all draws are 64-bit then)")
     ap.add_argument("--spec-min-ctx", type=int, default=None,
                     help="rows with fewer cached tokens than this do not draft yet (0 = always)")
     ap.add_argument("--spec-sparse-k", type=int, default=0, help="approximate batched verify over the k best history blocks (refused when > 0: not built)")

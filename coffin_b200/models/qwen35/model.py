@@ -1366,6 +1366,14 @@ class Qwen35Model:
         u = torch.tensor(us, dtype=torch.float32, device=self.device)
         return K.sample(logits.contiguous(), t, u)
 
+    def draw(self, logits: torch.Tensor, temps: list[float], us: list[float]) -> torch.Tensor:
+        """``sample`` with the 64-bit draw of ``accept_tree`` (every row a tree of its root alone): the same logits and uniform give the
+        token that a tree step gives.  ``sample`` sums in 32 bits and draws another token in up to one of forty of its draws."""
+        M = logits.shape[0]
+        host = torch.tensor([temps, us], dtype=torch.float32).to(self.device)
+        roots = torch.ones(M, 1, dtype=torch.int64, device=self.device)
+        return tree.verify_tree(logits[:, None], roots, roots, host[0], host[1])[2]
+
     @staticmethod
     def bucket_for(n: int) -> int:
         for m in BUCKETS:

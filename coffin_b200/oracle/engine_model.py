@@ -281,6 +281,10 @@ class OracleEngineModel:
     def commit(self, slot: int, n_accept: int) -> None:
         self.commit_batch([slot], [n_accept])
 
+    def draw(self, logits: torch.Tensor, temps, us) -> torch.Tensor:
+        """The draw of ``accept_tree``; the twin's ``sample`` is 64-bit as well."""
+        return self.sample(logits, temps, us)
+
     def sample(self, logits: torch.Tensor, temps, us) -> torch.Tensor:
         """Greedy when ``temps`` is None; else per-row inverse-CDF sampling with uniforms ``us``
         (rows with temperature <= 0 stay greedy)."""

@@ -56,3 +56,37 @@ def test_the_device_model_verifies_trees_on_one_rank_only():
     comm = object()
     assert says(SimpleNamespace(tp=None, tp_world=1, ep_world=1)) and says(SimpleNamespace(tp=comm, tp_world=1, ep_world=1))
     assert not says(SimpleNamespace(tp=comm, tp_world=2, ep_world=1)) and not says(SimpleNamespace(tp=comm, tp_world=1, ep_world=2))
+
+
+class TwoSamplers(OracleEngineModel):
+    """A model whose plain draw differs from the draw of its tree pass."""
+
+    def sample(self, logits, temps, us):
+        out = super().sample(logits, temps, us)
+        if temps is None:
+            return out
+        self.plain = getattr(self, "plain", 0) + 1
+        return torch.tensor([(int(t) + (temp > 0)) % logits.shape[1] for t, temp in zip(out, temps)])
+
+    def draw(self, logits, temps, us):
+        self.drawn = getattr(self, "drawn", 0) + 1
+        return super().sample(logits, temps, us)
+
+
+@torch.no_grad()
+def test_a_sampled_request_has_one_sampler_whether_or_not_a_step_drafted():
+    """With speculation over trees every token of a request is drawn alike: the first one, those of steps without drafts and those of tree
+    steps.  Without it the plain draw is used, as ever."""
+    prompts = [_repetitive(4), _repetitive(5, 50)]
+    params = [SamplingParams(max_tokens=24, temperature=0.05, seed=3), SamplingParams(max_tokens=24, temperature=0.9, seed=5)]
+    ref = [_engine().generate([p], q)[0].output for p, q in zip(prompts, params)]        # the oracle's draws throughout
+    for kw in ({"spec_sample": True}, {"spec_tree": 7}, {"spec_tree": 7, "spec_sample": True}):
+        eng = _engine(TwoSamplers, spec_k=3, spec_batch=True, **kw)
+        seqs = [eng.add_request(p, q) for p, q in zip(prompts, params)]
+        while any(not s.finished for s in seqs):
+            eng.step()
+        assert [s.output for s in seqs] == ref, kw
+        assert not hasattr(eng.model, "plain") and eng.model.drawn > 0
+    eng = _engine(TwoSamplers, spec_k=3, spec_batch=True)
+    eng.generate(prompts[:1], params[0])
+    assert eng.model.plain > 0 and not hasattr(eng.model, "drawn")
