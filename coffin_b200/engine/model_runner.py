@@ -381,7 +381,11 @@ class ModelRunner:
             if s.drafter_seen < len(toks):
                 s.drafter.observe(toks[s.drafter_seen:])
                 s.drafter_seen = len(toks)
-            trees.append(s.drafter.draft_tree(k, min(room, self.cfg.spec_tree if self.cfg.spec_tree > 0 else k)))
+            if self.cfg.spec_tree > 0:
+                trees.append(s.drafter.draft_tree(k, min(room, self.cfg.spec_tree)))
+            else:
+                chain = s.drafter.draft(min(k, room))
+                trees.append((chain, list(range(-1, len(chain) - 1))))
         return trees if any(t for t, _p in trees) else None
 
     def tree_step(self, seqs: list[Sequence], tokens: list[int], trees: list[tuple[list[int], list[int]]]) -> list[list[int]]:

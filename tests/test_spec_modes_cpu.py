@@ -90,3 +90,18 @@ def test_a_sampled_request_has_one_sampler_whether_or_not_a_step_drafted():
     eng = _engine(TwoSamplers, spec_k=3, spec_batch=True)
     eng.generate(prompts[:1], params[0])
     assert eng.model.plain > 0 and not hasattr(eng.model, "drawn")
+
+
+@torch.no_grad()
+def test_without_a_number_of_tree_nodes_a_row_drafts_one_chain():
+    """Continuations that end with the history leave room for others, which branch where the tree flag is set and nowhere else."""
+    prompt = [5, 6, 7, 8, 9, 5, 6, 7, 8, 1, 2, 5, 6, 7, 8, 1, 5, 6]
+    for q in (SamplingParams(max_tokens=4), SamplingParams(max_tokens=4, temperature=0.5, seed=1)):
+        drafted = {}
+        for n in (0, 12):
+            eng = _engine(spec_k=7, spec_sample=True, spec_tree=n)
+            seq = eng.add_request(prompt, q)
+            (drafted[n],) = eng.runner.draft_trees([seq])
+        tokens, parents = drafted[0]
+        assert tokens == [7, 8, 1, 5, 6] == seq.drafter.draft(7) and parents == [-1, 0, 1, 2, 3]
+        assert drafted[12][0][:5] == tokens and len(drafted[12][0]) > 5
