@@ -896,7 +896,9 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
     }
   }
   l = warp_sum(l);
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  // no weight at all: 0.  (A sum that is no number reaches the row whatever the partial sums that were skipped: scores of a whole piece that
+  // are NaN leave its maximum at -inf.)
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   bf16* op = a.out + row * a.ldo + (int64_t)h * HD + lane * EPL;
 #pragma unroll
   for (int e = 0; e < EPL; ++e) o[e] *= inv * (a.gate ? sigmoid_f(gp.at(e)) : 1.f);

@@ -117,7 +117,8 @@ def attn_tree(q, proj, kpool, vpool, block_tables, positions, anc, out, *, nh: i
     """Attention of tree nodes over their sequences' pages and their own paths: ``q [R * C, nh, hd]`` normed and rotated, the nodes'
     keys and values in the pools already; ``proj`` supplies the output gate as for ``kernels.attn_prefill`` (``None``: no gate).
     ``block_tables [R, pages]`` and ``positions [R]`` (cached tokens, < 0: unused row) int32; rows without a node stay as they were.
-    ``kscale`` / ``vscale``: the pools are int8."""
+    ``kscale`` / ``vscale``: the pools are int8.  Scores that are NaN or +inf make a row NaN; a row whose scores are all -inf, or that sees
+    no page, is 0."""
     R, C = _rows(anc)
     nh, nkv, hd = int(nh), int(nkv), int(hd)
     if hd not in (64, 128, 256) or nkv < 1 or nh < 1 or nh % nkv:

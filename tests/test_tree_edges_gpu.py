@@ -1,0 +1,64 @@
+"""Tree operators where numbers end: scores that are infinite or none, keys that are nearly equal, positions at the end of their type."""
+import math
+
+import pytest
+import torch
+
+import plain_tree as P
+from test_tree_gpu import Attn
+
+pytestmark = pytest.mark.gpu
+BF, F32, F64, I32, I64 = torch.bfloat16, torch.float32, torch.float64, torch.int32, torch.int64
+NAN, INF = float("nan"), float("inf")
+
+# (contexts, nodes, heads, kv heads, head width): a page a piece, pieces of several pages, pairs of CTAs
+SHAPES = [([200, 100], 3, 8, 2, 64), ([20000, 70], 4, 16, 4, 256), ([900, 300], 48, 8, 2, 128)]
+
+
+def _page_rows(a, r, pages):
+    """Pool rows of the cached tokens in these pages of sequence r."""
+    return torch.tensor([s for s in P.slots_of(a.tables[r].tolist(), range(a.contexts[r]))], device="cuda").split(64)[pages[0]:pages[1]]
+
+
+@pytest.mark.parametrize("q8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("shape", SHAPES, ids=["page", "pages", "pairs"])
+@pytest.mark.parametrize("pages", [(1, 2), (0, 1), (0, 10000)], ids=["second", "first", "all"])
+def test_scores_that_are_no_numbers_reach_the_output(shape, pages, q8):
+    """Whole pages of keys that are NaN, alone or with the rest of the cache: the sequence's rows are NaN, the other's stay as they were."""
+    contexts, C, nh, nkv, hd = shape
+    a = Attn(2, C, contexts, nh, nkv, hd, q8, seed=31)
+    a.run()
+    healthy = a.out.clone()
+    rows = torch.cat(_page_rows(a, 0, pages))
+    if q8:
+        a.kscale[rows] = NAN
+    else:
+        a.kpool[rows] = NAN
+    a.run()
+    assert a.out[:C].isnan().all()
+    assert torch.equal(a.out[C:], healthy[C:])
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=["page", "pages", "pairs"])
+def test_infinite_scores(shape):
+    """A score of -inf is a weight of 0; +inf makes the row NaN, as inf - inf does; a row whose scores are all -inf is 0, like one that
+    sees no key."""
+    contexts, C, nh, nkv, hd = shape
+    a = Attn(2, C, contexts, nh, nkv, hd, seed=32)
+    a.q.abs_().clamp_(min=0.01)                            # q.k has the sign of an infinite key
+    keys, tables = a.kpool.clone(), a.tables.clone()
+    rows = torch.cat(_page_rows(a, 0, (1, 2)))
+    a.tables[0, 1] = -1                                    # a page that is none leaves the sum: the same weights
+    a.run()
+    without = a.out.clone()
+    a.tables.copy_(tables)
+    a.kpool[rows] = -INF
+    a.run()
+    assert torch.equal(a.out, without)
+    a.kpool[rows[5]] = INF
+    a.run()
+    assert a.out[:C].isnan().all() and torch.equal(a.out[C:], without[C:])
+    a.kpool.copy_(keys)
+    a.kpool[P.slots_of(a.tables[0].tolist(), range(contexts[0] + C))] = -INF
+    a.run()
+    assert (a.out[:C] == 0).all() and torch.equal(a.out[C:], without[C:])
