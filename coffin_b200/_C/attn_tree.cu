@@ -54,9 +54,9 @@ struct TreeAttnArgs {
 __device__ __forceinline__ int cached_keys(const TreeAttnArgs& a, int r) { return max(0, min(a.positions[r], a.width * kPage)); }
 __device__ __forceinline__ int pages_of(int pos0, int width) { return (max(0, min(pos0, width * kPage)) + kPage - 1) / kPage; }
 __device__ __forceinline__ int cached_pages(const TreeAttnArgs& a, int r) { return pages_of(a.positions[r], a.width); }
-// first slot of a page, or -1 where the table names none of the pool's
-__device__ __forceinline__ int64_t page_slot(const TreeAttnArgs& a, int r, int page) {
-  if (page >= a.width) return -1;
+// First slot of a page, or -1 where the table names none of the pool's.  Pages of nodes come from positions that may pass 2^31: unsigned.
+__device__ __forceinline__ int64_t page_slot(const TreeAttnArgs& a, int r, unsigned page) {
+  if (page >= (unsigned)a.width) return -1;
   const int id = a.tables[(int64_t)r * a.ldbt + page];
   return (unsigned)id < (unsigned)a.pages ? (int64_t)id * kPage : -1;
 }
@@ -773,7 +773,7 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
   const int kvh = h / a.rep;
   int64_t slot0[2];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) slot0[u] = on >> (lane + 32 * u) & 1 ? page_slot(a, r, (pos0 + lane + 32 * u) / kPage) : -1;
+  for (int u = 0; u < 2; ++u) slot0[u] = on >> (lane + 32 * u) & 1 ? page_slot(a, r, ((unsigned)pos0 + lane + 32 * u) / kPage) : -1;
   // the cache's partials: maxima and sums, one a lane
   auto pieces = [&](int pos) { const int n = pages_of(pos, a.width); return L ? (n + L - 1) / L : n; };
   int all = pieces(mine0), before = lane < r ? all : 0;
@@ -804,7 +804,7 @@ __global__ void __launch_bounds__(256) tree_finish_kernel(const TreeAttnArgs a) 
   uint64_t path = 0;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    kr[u] = slot0[u] < 0 ? 0 : (slot0[u] + (pos0 + lane + 32 * u) % kPage) * a.nkv + kvh;
+    kr[u] = slot0[u] < 0 ? 0 : (slot0[u] + ((unsigned)pos0 + lane + 32 * u) % kPage) * a.nkv + kvh;
     if (Q8 && slot0[u] >= 0) { ks[u] = a.kscale[kr[u]]; vs[u] = a.vscale[kr[u]]; }
     path |= (uint64_t)__ballot_sync(0xffffffffu, slot0[u] >= 0) << (32 * u);
   }

@@ -26,8 +26,8 @@ __global__ void __launch_bounds__(256) kv_tree_commit_kernel(const KvCommitArgs 
   if (pos0 < 0 || n < 2) return;
   const int* table = a.tables + (int64_t)r * a.ldbt;
   const int* path = a.path + (int64_t)r * a.C;
-  auto slot = [&](int p) -> int64_t {
-    if (p / kPage >= a.width) return -1;
+  auto slot = [&](unsigned p) -> int64_t {                  // a position behind the cache may pass 2^31
+    if (p / kPage >= (unsigned)a.width) return -1;
     const int64_t s = (int64_t)table[p / kPage] * kPage + p % kPage;
     return s >= 0 && s < a.slots ? s : -1;
   };
@@ -43,8 +43,8 @@ __global__ void __launch_bounds__(256) kv_tree_commit_kernel(const KvCommitArgs 
       const int step = i0 + i, node = step < n ? path[step] : -1;
       to[i] = -1;
       if (node <= step || node >= a.C) continue;           // in place already (or no node)
-      const int64_t from = slot(pos0 + node);
-      to[i] = from < 0 ? -1 : slot(pos0 + step);
+      const int64_t from = slot((unsigned)pos0 + node);
+      to[i] = from < 0 ? -1 : slot((unsigned)pos0 + step);
       if (to[i] < 0) continue;
       if (scales) v[i].x = __float_as_uint(a.scale[which][(l * a.slots + from) * a.nkv + c - a.chunks]);
       else v[i] = *reinterpret_cast<const uint4*>(a.pool[which] + ((l * a.slots + from) * a.chunks + c) * 16);

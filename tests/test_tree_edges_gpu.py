@@ -62,3 +62,31 @@ def test_infinite_scores(shape):
     a.kpool[P.slots_of(a.tables[0].tolist(), range(contexts[0] + C))] = -INF
     a.run()
     assert (a.out[:C] == 0).all() and torch.equal(a.out[C:], without[C:])
+
+
+@pytest.mark.parametrize("q8", [False, True], ids=["bf16", "int8"])
+def test_positions_at_the_end_of_their_type(q8):
+    """Nodes whose positions pass 2^31 have no page, like those behind the table's last one: the row sees the table's pages alone, and a commit
+    moves nothing."""
+    from coffin_b200.ops import tree
+    last = 2 ** 31 - 1
+    a = Attn(4, 64, [100, 130, 70, 5], 8, 2, 64, q8, seed=33)
+    wide = a.tables.shape[1] * 64
+    a.tables[a.tables == 0] = -1                           # places behind a sequence's own pages: none of the pool's
+    a.positions.copy_(torch.tensor([wide, wide, wide, 5], dtype=I32))
+    a.run()
+    at_end = a.out.clone()
+    for back in (0, 1, 40, 62, 63, 64):
+        a.positions.copy_(torch.tensor([last - back, last, last - 31, 5], dtype=I32))
+        a.out.fill_(7.0)
+        a.run()
+        assert torch.equal(a.out, at_end), back
+    path = torch.arange(64, dtype=I32, device="cuda").repeat(4, 1)
+    path[:, 1:33] = torch.arange(2, 66, 2, dtype=I32, device="cuda").clamp(max=63)
+    steps = torch.tensor([33, 33, 33, 0], dtype=I32, device="cuda")
+    pools = [a.kpool[None].clone(), a.vpool[None].clone()]
+    scales = [a.kscale[None].clone(), a.vscale[None].clone()] if q8 else [None, None]
+    tree.kv_tree_commit(*pools, a.tables, a.positions, path, steps, *scales)
+    assert torch.equal(pools[0][0], a.kpool) and torch.equal(pools[1][0], a.vpool)
+    if q8:
+        assert torch.equal(scales[0][0], a.kscale) and torch.equal(scales[1][0], a.vscale)
