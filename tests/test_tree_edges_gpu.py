@@ -1,11 +1,10 @@
 """Tree operators where numbers end: scores that are infinite or none, keys that are nearly equal, positions at the end of their type."""
-import math
-
 import pytest
 import torch
 
 import plain_tree as P
-from test_tree_gpu import Attn
+import plain_tree_matrix as M
+from test_tree_gpu import Attn, Gdn
 
 pytestmark = pytest.mark.gpu
 BF, F32, F64, I32, I64 = torch.bfloat16, torch.float32, torch.float64, torch.int32, torch.int64
@@ -90,3 +89,25 @@ def test_positions_at_the_end_of_their_type(q8):
     assert torch.equal(pools[0][0], a.kpool) and torch.equal(pools[1][0], a.vpool)
     if q8:
         assert torch.equal(scales[0][0], a.kscale) and torch.equal(scales[1][0], a.vscale)
+
+
+@pytest.mark.parametrize("noise", [0.0, 0.02], ids=["equal", "near"])
+@pytest.mark.parametrize("C,nk,nv,d,kind", [(8, 2, 4, 128, "chain"), (8, 2, 4, 64, "star"), (24, 8, 32, 128, "chain"), (64, 8, 32, 128, "chain"), (64, 8, 64, 128, "tree"),
+                                            (64, 10, 80, 128, "chain"), (33, 10, 160, 128, "chain"), (64, 2, 4, 64, "chain")])
+def test_delta_net_of_a_run_of_one_token(C, nk, nv, d, kind, noise):
+    """Keys that are equal or nearly so, hardly any decay and every strength of update: the triangular inverse at its worst."""
+    a = Gdn(1, C, nk, nv, d, [20], kind, seed=C + nv)
+    conv = 2 * nk * d + nv * d
+    one = a.proj[:1].clone()
+    a.proj.copy_((one.float() * (1 + noise * torch.randn(a.proj.shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(5)))).to(BF))
+    a.ring[a.slots[0]] = one[0, :conv]
+    a.proj[:, conv + nv * d:conv + nv * d + nv] = torch.linspace(-3, 9, nv, device="cuda").to(BF)
+    a.A_log.fill_(-6.0)
+    a.run()
+    dims = a.dims
+    out, bound, D, De = M.gdn(a.proj[:, :a.width], a.conv_w, a.A_log, a.dt_bias, a.norm_w, a.ring[a.slots[0]], a.state[a.slots[0]], 20, a.parents[0], *dims, 1e-6)
+    for name, got, want, most in (("update", a.record[0, :, :, d:2 * d], D, De), ("out", a.out.view(C, nv, d), out, bound)):
+        off = (got.double() - want).abs()
+        assert float((off / most).max()) <= 1.0, name
+    # worst-case sums of signs over 64 equal keys; the node-by-node bound is 10^13 times the updates there
+    assert float((De / D.abs().amax((0, 2), keepdim=True)).max()) < 0.25
