@@ -15,7 +15,8 @@
 // page, the even one issues the products, and what those threads wait for is signalled there by both.  (Two items of 128 rows bring every
 // page twice: 2 x 64 nodes behind 65536 tokens 193 us, in pairs 149.)
 // What bounds it: 8 x 16 nodes behind 517 to 16391 tokens, 280 MB in 52 us, 5.4 TB/s, the rest are the ends of the pieces and the merge; 2 x 64
-// nodes behind 65536 tokens, 540 MB and 137 GFLOP in 110 us, tensor pipe 67 % busy; int8 pages, the issue slots that softmax and conversion share.
+// nodes behind 65536 tokens, 540 MB and 137 GFLOP in 119 us, tensor pipe 67 % busy; int8 pages, the chain of waits of a page (conversion, scores,
+// softmax, values: 1.6 us, a page at a time; issue slots 33 % and tensor pipe 24 % busy).
 //   warp 0       TMA: K and V pages into rings (a page of a kv head is a [64 x hd] box of the pool, hd / 64 swizzled [64 x 128 B] blocks)
 //   warp 1, 10   tcgen05.mma (one thread each): S = Q K^T with Q in tensor memory into one of two accumulators; O += P V
 //   warps 2-9    two groups of 128 threads, a thread a row: one takes the even pages, the other the odd ones, so that the exponentials of a
@@ -653,7 +654,7 @@ tree_cache_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant
                 p1 = tree_ex2(p1);
                 l2 = add2(l2, pack2(p0, p1));
                 if (Q8) unpack2(mul2(pack2(p0, p1), vs2[(c0 + k) / 2]), p0, p1);
-                pk[i] = pack_bf162(p0, p1);           // weights rounded to bf16, half a step 2^-8; their sum is not
+                pk[i] = pack_bf162(p0, p1);           // bf16, half a step 2^-8: the product takes operands of one type, and V is bf16; the sum is of the exact ones
               }
               *reinterpret_cast<uint4*>(prow + (((c0 / 8 + c) ^ (r & 7)) << 4)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
             }

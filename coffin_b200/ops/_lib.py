@@ -115,5 +115,6 @@ def exported() -> list[str]:
 
 def set_pdl(on: bool) -> None:
     """Launch kernels with programmatic dependent launch (the prologue of kernel n+1 overlaps
-    the tail of kernel n)."""
+    the tail of kernel n).  The switch concerns kernels of different operators: the second kernel of an operator of two
+    (``ops/tree.py``) always overlaps the first, whose results it waits for."""
     call_nostream("set_pdl", int(on))

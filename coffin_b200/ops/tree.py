@@ -214,7 +214,8 @@ def verify_tree(logits, tokens, anc, temperature, u) -> tuple[torch.Tensor, torc
     (lowest index) where the temperature is not positive; from node 0 on the first child that carries the token (``tokens [R, C]``
     int64) is next.  Returns ``path`` (int32 ``[R, C]``, -1 behind its end), ``steps`` (int32 ``[R]``, nodes on the path) and ``next``
     (int64 ``[R]``, the token drawn at its end): the new tokens are those of the path behind node 0, then ``next``, the ones that
-    sampling one by one with the same uniforms draws.  Draws are 64-bit.  A sequence whose node 0 is none gets 0 steps and token -1."""
+    one-node trees draw one by one with the same uniforms.  Draws are 64-bit (``kernels.sample`` sums in 32 bits and draws another token in
+    0.3 to 2.6 % of 151936-token draws).  A sequence whose node 0 is none gets 0 steps and token -1."""
     R, C = _rows(anc)
     lp, lds, ldr, V = _logits(logits, R, C)
     tp, Tp, up = _vec(tokens, R * C, _I64, "tokens"), _vec(temperature, R, _F32, "temperature"), _vec(u, R * C, _F32, "u")
@@ -274,7 +275,8 @@ def _path(path: torch.Tensor) -> torch.Size:
 def kv_tree_commit(kpool, vpool, block_tables, positions, path, steps, kscale=None, vscale=None) -> None:
     """Keys and values of the accepted paths move to consecutive positions, in all layers at once: the row at ``positions[r] + path[r, i]``
     to ``positions[r] + i`` for ``i < steps[r]``.  ``kpool`` / ``vpool [layers, slots, nkv, hd]`` (with ``kscale`` / ``vscale [layers, slots, nkv]``
-    int8), ``path`` and ``steps`` as :func:`verify_tree` returns them; a path's nodes are in increasing order."""
+    int8), ``path`` and ``steps`` as :func:`verify_tree` returns them (node 0 first, in increasing order).  Pages that are
+    written belong to one sequence alone."""
     R, C = _path(path)
     size, kv = kpool.shape, kpool.dtype
     if len(size) != 4 or vpool.shape != size or kv is not vpool.dtype or not kpool.is_contiguous() or not vpool.is_contiguous():
