@@ -329,9 +329,13 @@ class ModelRunner:
         from ..utils.suffix import SuffixDrafter
         if len(seqs) > self.SPEC_MAX_ROWS or not (self.cfg.spec_batch or len(seqs) == 1):
             return None
+        rows = 1
+        while rows < len(seqs):
+            rows *= 2
+        most = getattr(self.model, "verify_rows", 64) // rows - 1     # drafts a row that one pass over all rows has room for
         drafts, any_draft = [], False
         for s in seqs:
-            k = self.spec_k_of(s)
+            k = min(self.spec_k_of(s), most)
             if k <= 0:
                 drafts.append([])
                 continue

@@ -1053,6 +1053,11 @@ class Qwen35Model:
     # ------------------------------------------------------------------ speculative verification
     VERIFY_WIDTHS = (2, 4, 8)
 
+    @property
+    def verify_rows(self) -> int:
+        """Token rows of one verify pass; more than the decode projections carry are single-GPU."""
+        return WIDE if self.tp is not None and (self.tp_world > 1 or self.ep_world > 1) else BUCKETS[-1]
+
     def _verify_buffers(self, R: int, C: int) -> dict:
         """Buffers of a verify pass over ``R`` sequences x ``C`` tokens (``R`` a power of two)."""
         key = ("verify", R, C)
@@ -1104,7 +1109,7 @@ class Qwen35Model:
         N = R * C
         if N > BUCKETS[-1]:
             raise ValueError(f"{n} rows x {C} tokens exceed the {BUCKETS[-1]} token rows of one verify pass")
-        if N > WIDE and self.tp is not None and (self.tp_world > 1 or self.ep_world > 1):
+        if N > self.verify_rows:
             raise NotImplementedError("a verify pass of more than 8 token rows is single-GPU")
         tables = []
         for toks, pos0, slot, table, delta in rows:

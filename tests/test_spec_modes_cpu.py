@@ -105,3 +105,55 @@ def test_without_a_number_of_tree_nodes_a_row_drafts_one_chain():
         tokens, parents = drafted[0]
         assert tokens == [7, 8, 1, 5, 6] == seq.drafter.draft(7) and parents == [-1, 0, 1, 2, 3]
         assert drafted[12][0][:5] == tokens and len(drafted[12][0]) > 5
+
+
+class FewRows(ChainsOnly):
+    """Over several ranks a verify pass has at most 8 token rows, of a power of two of sequences."""
+    verify_rows = 8
+    widest = 0
+
+    def verify_batch(self, rows):
+        n = 1
+        while n < len(rows):
+            n *= 2
+        if n * len(rows[0][0]) > 8:
+            raise NotImplementedError("a verify pass of more than 8 token rows is single-GPU")
+        self.widest = max(self.widest, n * len(rows[0][0]))
+        return super().verify_batch(rows)
+
+
+class Knowing:
+    """Drafts a request's own tokens, so that chains are as long as they may be."""
+
+    def __init__(self, prompt, output):
+        self.want, self.seen = list(prompt) + list(output), 0
+
+    def observe(self, tokens):
+        self.seen += len(tokens)
+
+    def draft(self, k):
+        return self.want[self.seen:self.seen + k]
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("n", [1, 2, 3, 4])
+@pytest.mark.parametrize("kw", [{}, {"spec_tree": 9}], ids=["chain", "tree"])
+def test_chains_of_several_rows_fit_the_verify_pass_of_the_model(n, kw):
+    prompts = [_repetitive(20 + i, 48 + i) for i in range(n)]
+    ref = [_engine().generate([p], SamplingParams(max_tokens=12))[0].output for p in prompts]
+    eng = _engine(FewRows, spec_k=7, spec_batch=True, **kw)
+    seqs = [eng.add_request(p, SamplingParams(max_tokens=12)) for p in prompts]
+    for s, r in zip(seqs, ref):
+        s.drafter, s.drafter_seen = Knowing(s.prompt, r), 0
+    while any(not s.finished for s in seqs):
+        eng.step()
+    assert [s.output for s in seqs] == ref
+    assert eng.model.widest == 8 and eng.runner.stats()["spec"]["accepted"] > 0
+
+
+def test_rows_of_a_verify_pass_on_the_device():
+    from coffin_b200.models.qwen35.model import Qwen35Model
+    says = Qwen35Model.verify_rows.fget
+    comm = object()
+    assert says(SimpleNamespace(tp=None, tp_world=1, ep_world=1)) == 64 == says(SimpleNamespace(tp=comm, tp_world=1, ep_world=1))
+    assert says(SimpleNamespace(tp=comm, tp_world=2, ep_world=1)) == 8 == says(SimpleNamespace(tp=comm, tp_world=1, ep_world=2))
